@@ -160,6 +160,7 @@ def prepare(case, seed):
         s.q_rope = randn(sum(new), H, ROPE)
         s.kv = randn(sum(total), H, NOPE + VALUE)
         s.k_rope = randn(sum(total), ROPE)
+        s.most_new, s.most_keys = max(new), max(total)
         s.cu_q = _ints([sum(new[:i]) for i in range(len(new) + 1)])
         s.cu_k = _ints([sum(total[:i]) for i in range(len(new) + 1)])
     elif kind == "append":
@@ -201,22 +202,15 @@ def _run_own(s):
     return s.cache
 
 
-def _attend(q, keys, values, limits):
-    """q [S, H, d], keys [t, d] or [H, t, d], values alike, limits: positions that a row of queries sees -> out [S, H, dv], lse [S, H]."""
-    shared = keys.dim() == 2
-    scores = (torch.matmul(q, keys.t()) if shared else torch.matmul(q.transpose(0, 1), keys.transpose(1, 2)).transpose(0, 1)) * SCALE
-    hidden = torch.arange(scores.shape[-1], device=q.device)[None, :] >= limits[:, None]
-    scores = scores.masked_fill(hidden[:, None, :], float("-inf"))
+def _softmax_sum(scores, hidden, values):
+    """scores and hidden [.., rows, keys], values [.., keys, dv] -> out and the logarithm of the sum; rows that see nothing: 0, -inf."""
+    scores = scores.masked_fill(hidden, float("-inf"))
     top = scores.amax(-1, keepdim=True)
-    p = torch.exp(scores - top)
+    empty = top == float("-inf")
+    p = torch.exp(scores - top.masked_fill(empty, 0.0))
     total = p.sum(-1, keepdim=True)
-    out = (torch.matmul(p, values) if shared else torch.matmul(p.transpose(0, 1), values).transpose(0, 1)) / total
-    return out, (top + torch.log(total)).squeeze(-1)
-
-
-def _rows(cache, table, n):
-    page = cache.shape[1]
-    return cache[table[:-(-n // page)].long()].flatten(0, 1)[:n]
+    out = torch.matmul(p, values) / total.masked_fill(empty, 1.0)
+    return out, (top + torch.log(total.masked_fill(empty, 1.0))).squeeze(-1)
 
 
 def _rotate(x, positions, inv_freq):
@@ -229,40 +223,55 @@ def _rotate(x, positions, inv_freq):
     return torch.stack([a * cos - b * sin, a * sin + b * cos], -1).flatten(-2)
 
 
+def _plain_decode(s):
+    """The batch padded to its longest sequence: a shared prefix is one more block of keys in front of each sequence's own."""
+    B, S, H, R = s.q_latent.shape
+    page = s.cache.shape[1]
+    device = s.cache.device
+    keys = s.cache[s.table.long()].flatten(1, 2)
+    at = torch.arange(keys.shape[1], device=device).expand(B, -1)
+    length, there = s.lens.long()[:, None], at < s.lens[:, None]
+    if s.kind == "shared":
+        group = torch.searchsorted(s.starts, torch.arange(B, device=device, dtype=torch.int32), right=True) - 1
+        before = s.prefix_lens.long()[group][:, None]
+        keys = torch.cat([s.cache[s.prefix_table.long()[group]].flatten(1, 2), keys], 1)
+        first = torch.arange(s.prefix_table.shape[1] * page, device=device).expand(B, -1)
+        at, there = torch.cat([first, at + before], 1), torch.cat([first < before, there], 1)
+        length = length + before
+    limits = length - (S - 1) + torch.arange(S, device=device)
+    hidden = ~there[:, None, :] | (at[:, None, :] >= limits[:, :, None])  # [B, S, keys]
+    keys = keys.float()
+    q = torch.cat([s.q_latent, s.q_rope], -1).float().flatten(1, 2)
+    scores = torch.matmul(q, keys.transpose(1, 2)) * SCALE
+    out, lse = _softmax_sum(scores, hidden.repeat_interleave(H, 1), keys[..., :R])
+    return out.view(B, S, H, R).to(s.q_latent.dtype), lse.view(B, S, H)
+
+
+def _plain_prefill(s):
+    """The prompts padded to the longest."""
+    device = s.q.device
+    cu_q, cu_k = s.cu_q.long(), s.cu_k.long()
+    new, total = cu_q.diff()[:, None], cu_k.diff()[:, None]
+    i, j = torch.arange(s.most_new, device=device), torch.arange(s.most_keys, device=device)
+    rows = (cu_q[:-1, None] + i).clamp(max=s.q.shape[0] - 1)
+    keys = (cu_k[:-1, None] + j).clamp(max=s.kv.shape[0] - 1)
+    q = torch.cat([s.q[..., :NOPE], s.q_rope], -1)[rows].float().transpose(1, 2)
+    kv = s.kv[keys].float().transpose(1, 2)
+    rope = s.k_rope[keys].float()[:, None].expand(-1, kv.shape[1], -1, -1)
+    scores = torch.matmul(q, torch.cat([kv[..., :NOPE], rope], -1).transpose(-1, -2)) * SCALE
+    hidden = (j[None, None, :] >= (total - new + 1 + i)[:, :, None]) | (j >= total)[:, None, :]
+    out, lse = _softmax_sum(scores, hidden[:, None], kv[..., NOPE:])
+    row = torch.arange(s.q.shape[0], device=device)
+    seq = torch.searchsorted(cu_q, row, right=True) - 1
+    row = row - cu_q[seq]
+    return out[seq, :, row].to(s.q.dtype), lse[seq, :, row]
+
+
 def _run_plain(s):
     if s.kind in ("decode", "shared"):
-        B, S, H, R = s.q_latent.shape
-        q = torch.cat([s.q_latent.float(), s.q_rope.float()], -1)
-        outs, lses = [], []
-        lens = s.lens.tolist()
-        if s.kind == "shared":
-            starts, prefix = s.starts.tolist(), s.prefix_lens.tolist()
-        for b in range(B):
-            rows, n = _rows(s.cache, s.table[b], lens[b]), lens[b]
-            if s.kind == "shared":
-                g = max(i for i in range(len(prefix)) if starts[i] <= b)
-                rows, n = torch.cat([_rows(s.cache, s.prefix_table[g], prefix[g]), rows]), n + prefix[g]
-            limits = n - (S - 1) + torch.arange(S, device=q.device)
-            rows = rows.float()
-            out, lse = _attend(q[b], rows, rows[:, :R], limits)
-            # a draft longer than its sequence: the rows before its first position see nothing
-            empty = limits <= 0
-            outs.append(out.masked_fill(empty[:, None, None], 0.0))
-            lses.append(lse.masked_fill(empty[:, None], float("-inf")))
-        return torch.stack(outs).to(s.q_latent.dtype), torch.stack(lses)
+        return _plain_decode(s)
     if s.kind == "prefill":
-        cu_q, cu_k = s.cu_q.tolist(), s.cu_k.tolist()
-        q = torch.cat([s.q[..., :NOPE], s.q_rope], -1)
-        out = torch.empty(q.shape[0], q.shape[1], VALUE, dtype=q.dtype, device=q.device)
-        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
-        for i in range(len(cu_q) - 1):
-            q0, q1, k0, k1 = cu_q[i], cu_q[i + 1], cu_k[i], cu_k[i + 1]
-            limits = (k1 - k0) - (q1 - q0) + 1 + torch.arange(q1 - q0, device=q.device)
-            for h in range(q.shape[1]):
-                keys = torch.cat([s.kv[k0:k1, h, :NOPE].float(), s.k_rope[k0:k1].float()], -1)
-                o, l = _attend(q[q0:q1, h:h + 1].float(), keys, s.kv[k0:k1, h, NOPE:].float(), limits)
-                out[q0:q1, h:h + 1], lse[q0:q1, h:h + 1] = o.to(out.dtype), l
-        return out, lse
+        return _plain_prefill(s)
     if s.kind == "append":
         R = s.weight.shape[0]
         c = s.kv[:, :R].float()
