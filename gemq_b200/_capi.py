@@ -44,7 +44,21 @@ class MoeLayer(C.Structure):
                 ("s1", Single), ("s3", Single), ("s2", Single)]
 
 
-_P, _I, _Z = C.c_void_p, C.c_int, C.c_size_t
+_P, _I, _Z, _L, _F = C.c_void_p, C.c_int, C.c_size_t, C.c_int64, C.c_float
+
+
+class LatentDecode(C.Structure):
+    _fields_ = [("q_latent", _P), ("q_latent_stride", _L * 3), ("q_rope", _P), ("q_rope_stride", _L * 3), ("cache", _P),
+                ("page_stride", _L), ("n_pages", _I), ("page_size", _I), ("table", _P), ("table_pitch", _I), ("lens", _P),
+                ("prefix_table", _P), ("prefix_pitch", _I), ("prefix_lens", _P), ("starts", _P), ("groups", _I), ("batch", _I),
+                ("steps", _I), ("heads", _I), ("rank", _I), ("scale", _F), ("is_bf16", _I), ("out", _P), ("lse", _P), ("err", _P)]
+
+
+class LatentPrefill(C.Structure):
+    _fields_ = [("q_nope", _P), ("q_nope_stride", _L * 2), ("q_rope", _P), ("q_rope_stride", _L * 2), ("kv", _P), ("kv_stride", _L * 2),
+                ("k_rope", _P), ("k_rope_stride", _L), ("cu_q", _P), ("cu_k", _P), ("batch", _I), ("q_rows", _I), ("k_rows", _I),
+                ("heads", _I), ("causal", _I), ("scale", _F), ("is_bf16", _I), ("out", _P), ("lse", _P), ("err", _P)]
+
 
 _SIGNATURES = {
     "gemq_version": (C.c_char_p, []),
@@ -81,6 +95,11 @@ _SIGNATURES = {
     "gemq_step_gemv": (_I, [_P, _P, _I, _P, C.c_float, _P, _P, _I, _P, _I, _P, _I, _P, _I, _I, _P]),
     "gemq_step_norm": (_I, [_P, _P, _I, _P, C.c_float, _P, _P, _I, _I, _P]),
     "gemq_step_attention": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
+    "gemq_latent_append": (_I, [_P, _L, _P, _L, _L, _P, _F, _P, _F, _P, _P, _P, _L, _I, _I, _P, _P, _I, _I, _I, _I, _P, _P]),
+    "gemq_latent_decode_scratch_bytes": (_Z, [C.POINTER(LatentDecode)]),
+    "gemq_latent_decode": (_I, [C.POINTER(LatentDecode), _P, _Z, _P]),
+    "gemq_latent_prefill": (_I, [C.POINTER(LatentPrefill), _P]),
+    "gemq_copy_pages": (_I, [_P, _L, _L, _I, _I, _L, _P, _P, _I, _P, _P]),
     "gemq_moe_decode": (_I, [C.POINTER(MoeLayer), _P, _P, _P, _P, _I, _I, _I, _P, _Z, _P]),
 }
 

@@ -1,0 +1,54 @@
+// What the latent attention kernels share: 16-bit types, and where the rows of a sequence lie.
+#pragma once
+
+#include "common.cuh"
+
+namespace gemq {
+namespace latent {
+
+constexpr int kRope = 64;  // rotated part of a key
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+template <typename T> struct Pair;  // two 16-bit numbers in a word
+template <> struct Pair<__half> {
+  static constexpr int kBf16 = 0;
+  static __device__ __forceinline__ float2 f(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+  static __device__ __forceinline__ uint32_t r(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+template <> struct Pair<__nv_bfloat16> {
+  static constexpr int kBf16 = 1;
+  static __device__ __forceinline__ float2 f(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v)); }
+  static __device__ __forceinline__ uint32_t r(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+
+inline bool rank_ok(int rank) { return rank >= 128 && rank <= 512 && rank % 128 == 0; }
+inline bool page_ok(int page_size) { return page_size == 16 || page_size == 32 || (page_size > 0 && page_size % 64 == 0); }
+
+// A length as the device has it, within its table; one that is not is reported.
+__device__ __forceinline__ int clamp_length(int n, int pitch, int page_size, int* err) {
+  const long long most = static_cast<long long>(pitch) * page_size;
+  if (n >= 0 && n <= most) return n;
+  atomicExch(err, GEMQ_LATENT_BAD_LENGTH);
+  return n < 0 ? 0 : static_cast<int>(most);
+}
+
+// Entry i of n + 1 offsets that are meant to rise from 0 to at most `most`: where they do not, as if they did (every entry the largest
+// up to it, within 0 .. most).  By one thread, for checks; kernels scan.
+__device__ __forceinline__ bool offsets_ok(const int* v, int n, int most, bool to_the_end) {
+  int last = 0;
+  bool ok = v[0] == 0;
+  for (int i = 1; i <= n; ++i) {
+    ok = ok && v[i] >= last && v[i] <= most;
+    last = v[i];
+  }
+  return ok && (!to_the_end || last == most);
+}
+
+}  // namespace latent
+}  // namespace gemq

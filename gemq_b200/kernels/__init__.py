@@ -7,3 +7,4 @@ from .fused_dequant_bmm import (fused_dequant_down_proj, fused_dequant_down_proj
                                 fused_dequant_up_proj_triton)
 from .dequant_gemm import dequant_gemm, dequant_gemm_triton
 from .dequant_group_gemm import dequant_group_gemm, dequant_group_gemm_triton
+from .latent_attention import copy_pages, latent_append, latent_decode, latent_decode_shared, latent_error, latent_prefill

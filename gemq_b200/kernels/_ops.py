@@ -47,16 +47,16 @@ def _plain(args) -> bool:
     return True
 
 
-def library_op(name: str, fake, fast=None):
-    """``@library_op("name", fake_fn)``: register ``fn`` as ``gemq_b200::name`` (no argument is
-    mutated, outputs are fresh tensors) with ``fake_fn`` as its shape/dtype propagation.
+def library_op(name: str, fake, fast=None, mutates=()):
+    """``@library_op("name", fake_fn)``: register ``fn`` as ``gemq_b200::name`` (no argument but those named in
+    ``mutates`` is written, outputs are fresh tensors) with ``fake_fn`` as its shape/dtype propagation.
 
     A call in eager mode goes straight to ``fn``: the Python dispatch of a custom operator costs
     20-30 us of host time, more than the kernels of a small call take.  ``fast`` is tried before it with the
     positional arguments: native code that returns None for what it does not take.  Every other call
     (``plain_call``) is the operator."""
     def deco(fn):
-        op = torch.library.custom_op(f"{NAMESPACE}::{name}", mutates_args=())(fn)
+        op = torch.library.custom_op(f"{NAMESPACE}::{name}", mutates_args=mutates)(fn)
         op.register_fake(fake)
         overload = op._opoverload
 

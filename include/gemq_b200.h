@@ -313,6 +313,95 @@ int gemq_step_norm(const void* x, const void* res, int res_is_half, const void* 
 int gemq_step_attention(const void* qkv, const float* inv_freq, const int64_t* pos, void* keys, void* values, void* out,
                         int heads, int kv_heads, int head_dim, int cache_len, int is_bf16, gemq_stream_t stream);
 
+/* ---- latent attention over a paged cache ------------------------------------------------------- */
+
+/* No counterpart in the reference, which leaves the attention to the host model.  Every token is cached as one row of
+ * width rank + 64 that all heads share: the normalised latent vector c [rank] and the rotated key part k [64].  A cache is
+ * pages of page_size rows: row r of page p lies at cache + p * page_stride + r * (rank + 64) elements.  page_size is 16, 32 or a
+ * multiple of 64; rank is 128, 256, 384 or 512.  16-bit type T is fp16, or bf16 with is_bf16.  `err`: a device word that gets a code
+ * when the device data is out of range (GEMQ_LATENT_*); such entries are never used as an index.  */
+enum {
+  GEMQ_LATENT_BAD_PAGE = 41,   /* page id outside the cache: what would see the page is NaN, a copy is skipped */
+  GEMQ_LATENT_BAD_LENGTH = 42, /* negative length, or one beyond its page table: clamped; offsets that do not rise: as if they did */
+  GEMQ_LATENT_BAD_SLOT = 43,   /* slot outside the cache: the row is not stored (-1 is not an error) */
+  GEMQ_LATENT_WAIT = 44        /* a wait inside a kernel ran out */
+};
+
+/* rows [tokens, rank + 64] = { RMSNorm(kv[:, :rank]) * norm_weight, kv[:, rank:] rotated }, each rounded once to T, also stored at row
+ * slots[t] (page slots[t] / page_size; slots[t] < 0: not stored, -1 silently) of the cache; q_out [tokens, heads, 64] = q_rope rotated.
+ * Rotation of the pair (x[2i], x[2i+1]) by the angle positions[t] * inv_freq[i], formed in 64 bits, times rope_scale.  The strides
+ * are in elements, the last dimensions contiguous.  Slots that are stored to must be distinct.  kv, q_rope, norm_weight, cache,
+ * rows and q_out 16-byte aligned, strides multiples of 8 elements.  heads may be 0 (q_rope and q_out unused). */
+int gemq_latent_append(const void* kv, int64_t kv_stride, const void* q_rope, int64_t q_token_stride, int64_t q_head_stride,
+                       const void* norm_weight, float eps, const float* inv_freq, float rope_scale, const int64_t* positions,
+                       const int64_t* slots, void* cache, int64_t page_stride, int n_pages, int page_size, void* rows, void* q_out,
+                       int tokens, int heads, int rank, int is_bf16, int32_t* err, gemq_stream_t stream);
+
+/* Attention of `steps` query rows a sequence over its cached rows, the queries in the latent space:
+ *   s = scale * (q_latent . c + q_rope . k),  out [batch, steps, heads, rank] = softmax(s) c,  lse [batch, steps, heads] = log sum exp s.
+ * Sequence b has lens[b] cached rows, the pages table[b][..]; its query i sees those before position lens[b] - (steps - 1 - i).
+ * A row that sees nothing gives 0 and -inf.  With groups > 0 sequences starts[g] .. starts[g+1] - 1 have the prefix_lens[g] rows of
+ * pages prefix_table[g][..] in front of their own (lens and table count the own ones only); a group's prefix is read once
+ * for all its sequences.  starts[0] is 0 and starts[groups] is batch.
+ * q_latent and q_rope have strides (batch, step, head) in elements, multiples of 8, and 16-byte aligned beginnings; out
+ * and lse are contiguous. */
+typedef struct {
+  const void* q_latent;
+  int64_t q_latent_stride[3];
+  const void* q_rope;
+  int64_t q_rope_stride[3];
+  const void* cache;
+  int64_t page_stride;
+  int32_t n_pages, page_size;
+  const int32_t* table;        /* [batch, table_pitch] */
+  int32_t table_pitch;
+  const int32_t* lens;         /* [batch] */
+  const int32_t* prefix_table; /* [groups, prefix_pitch] */
+  int32_t prefix_pitch;
+  const int32_t* prefix_lens;  /* [groups] */
+  const int32_t* starts;       /* [groups + 1] */
+  int32_t groups;
+  int32_t batch, steps, heads, rank;
+  float scale;
+  int32_t is_bf16;
+  void* out;
+  float* lse;
+  int32_t* err;
+} gemq_latent_decode_t;
+size_t gemq_latent_decode_scratch_bytes(const gemq_latent_decode_t* args);
+int gemq_latent_decode(const gemq_latent_decode_t* args, void* scratch, size_t scratch_bytes, gemq_stream_t stream);
+
+/* Attention of whole prompts over expanded keys and values:
+ *   s = scale * (q_nope . kv[.., :128] + q_rope . k_rope),  out [q_rows, heads, 128] = softmax(s) kv[.., 128:],  lse [q_rows, heads].
+ * Sequence b has query rows cu_q[b] .. cu_q[b+1] - 1 and key rows cu_k[b] .. cu_k[b+1] - 1; its query i sees key j if
+ * j <= i + (keys - queries), or all keys without causal.  Rows that see nothing, and query rows behind the last sequence, give 0 and
+ * -inf.  Strides (row, head) in elements, multiples of 8, the last dimension contiguous, 16-byte aligned beginnings. */
+typedef struct {
+  const void* q_nope;          /* [q_rows, heads, 128] */
+  int64_t q_nope_stride[2];
+  const void* q_rope;          /* [q_rows, heads, 64] */
+  int64_t q_rope_stride[2];
+  const void* kv;              /* [k_rows, heads, 256] */
+  int64_t kv_stride[2];
+  const void* k_rope;          /* [k_rows, 64] */
+  int64_t k_rope_stride;
+  const int32_t* cu_q;         /* [batch + 1] */
+  const int32_t* cu_k;         /* [batch + 1] */
+  int32_t batch, q_rows, k_rows, heads, causal;
+  float scale;
+  int32_t is_bf16;
+  void* out;
+  float* lse;
+  int32_t* err;
+} gemq_latent_prefill_t;
+int gemq_latent_prefill(const gemq_latent_prefill_t* args, gemq_stream_t stream);
+
+/* Page dst[i] = page src[i] in each of `layers` caches of n_pages pages: page p of layer l is page_bytes bytes at
+ * cache + l * layer_stride + p * page_stride (bytes; page_bytes, strides and beginning multiples of 16).  The destinations must be
+ * distinct and no page may be both read and written, but for src[i] == dst[i], which is left alone. */
+int gemq_copy_pages(void* cache, int64_t layer_stride, int64_t page_stride, int layers, int n_pages, int64_t page_bytes, const int64_t* src,
+                    const int64_t* dst, int copies, int32_t* err, gemq_stream_t stream);
+
 /* ---- for callers that cannot allocate --------------------------------------------------------- */
 
 /* No counterpart in the reference.  y[1, N] = x[1, K] @ deq(wq), the same result as
