@@ -127,4 +127,19 @@ bool tensor_map_blocks(CUtensorMap* out, const void* base, int K, long long rows
   return true;
 }
 
+// Pages of 16-bit rows of `blocks` * 64 numbers as (64, row of a page, block, page): a box brings `box_rows` rows of a page, `box_blocks`
+// neighbouring blocks, each as swizzled rows of 128 bytes.  page_stride in elements.  Made anew for every call: about 0.3 us.
+bool tensor_map_pages(CUtensorMap* out, const void* base, int blocks, int page_size, long long page_stride, int pages, int box_rows,
+                      int box_blocks) {
+  EncodeTiledFn enc = encode_tiled_fn();
+  if (!enc) return false;
+  const cuuint64_t row = static_cast<cuuint64_t>(blocks) * 128;
+  const cuuint64_t dims[4] = {64, static_cast<cuuint64_t>(page_size), static_cast<cuuint64_t>(blocks), static_cast<cuuint64_t>(pages)};
+  const cuuint64_t strides[3] = {row, 128, pages > 1 ? static_cast<cuuint64_t>(page_stride) * 2 : row * page_size};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows), static_cast<cuuint32_t>(box_blocks), 1};
+  const cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
+  return enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }  // namespace gemq
