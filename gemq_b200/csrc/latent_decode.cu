@@ -12,12 +12,13 @@
 // of an MMA's 128, and 512 columns of results all of the tensor memory.)
 //
 // Persistent, one CTA an SM.  All row tiles of all sequences (and groups) times their 64-row tiles of the cache are one list, cut
-// into equal shares; a CTA's share is a run of pieces (row tile, range of tiles).  A piece that is all of a row tile is finished in
-// place, others leave their sums (fp32), maximum and sum of weights to the second kernel, which joins them in order of position.
-//   warp 0     TMA: a ring of blocks of 64 rows x 64 numbers, latent ones in pairs (2.75 tiles deep at N = 16), rope ones apart
-//   warp 1     MMA: S of tile k, then O of tile k - 1
-//   warps 2-3  the queries of the next piece into shared memory
-//   warps 4-7  softmax (a thread has two positions x N / 4 rows), O's correction, results
+// into shares of equal cost; a CTA's share is a run of pieces (row tile, range of tiles).  A piece that is all of a row tile is finished
+// in place, others leave their sums (fp32), maximum and sum of weights to the second kernel, which joins them in order of position.
+//   warp 0       TMA: a ring of blocks of 64 rows x 64 numbers, latent ones in pairs (2.75 tiles deep at N = 16), rope ones apart
+//   warps 1, 2   MMAs of S, of O.  (One warp for S of tile k + 1, then O of tile k: the latter waited for tile k + 1 to arrive, and the
+//                ring for it.)
+//   warps 4-7    softmax (a thread has two positions x N / 4 rows), O's correction
+//   warps 8-11   the queries of the next piece into shared memory, results of the last
 // The maximum that the weights refer to moves only when a row's scores exceed it by 2^8: O is corrected in tensor memory a few times per
 // sequence.  Rows behind what is seen are zeroed in shared memory before they are multiplied by weights of 0: what lies there may be NaN.
 // Every wait is bounded.
@@ -35,9 +36,11 @@ namespace {
 
 constexpr int kTile = 64;            // positions of a tile
 constexpr int kBlock = kTile * 128;  // bytes of 64 positions x 64 numbers
-constexpr int kThreads = 256;
-constexpr int kSoftWarp = 4;
-constexpr int kSlots = 16;           // tiles in flight that are told apart; the ring holds 11 at most (rank 128)
+constexpr int kThreads = 384;
+constexpr int kSoftWarp = 4, kEdgeWarp = 8;  // four each: a warp reads the quarter of the tensor memory that its number names
+// What a piece costs beside its tiles, in quarters of a tile.
+constexpr int kPieceCost = 4;
+constexpr int kSlots = 8;            // tiles in flight that are told apart: one more than the rope blocks, 4, at most
 
 // Blocks of the ring: what 227 KB hold beside the queries.
 template <int N> struct Ring;
@@ -45,20 +48,23 @@ template <> struct Ring<16> { static constexpr int kLatent = 22, kRopes = 3; };
 template <> struct Ring<32> { static constexpr int kLatent = 20, kRopes = 3; };
 template <> struct Ring<64> { static constexpr int kLatent = 16, kRopes = 2; };
 
-struct Start { int e, rt, t, left, rto; };
+struct Start { int e, rt, base, from, to, rto; };  // Walk's
 
 template <int N>
 struct Smem {
   static constexpr int kLatent = Ring<N>::kLatent, kRopes = Ring<N>::kRopes;
+  static constexpr int kOs = N <= 32 ? 2 : 1;  // accumulators that tensor memory holds
   alignas(1024) unsigned char ring[kLatent][kBlock];
   unsigned char rope[kRopes][kBlock];
   unsigned char q[9][N * 128];
   unsigned char p[N * 128];
-  float wmax[2][4][N];
+  float wmax[4][N];
   float fac[N];
-  alignas(8) unsigned long long full[kLatent / 2], rope_full[kRopes];
+  float2 result[N];  // reference and sum of the weights of the piece that is finished
+  int limit[N];
+  alignas(8) unsigned long long full[kLatent / 2], empty[kLatent / 2], rope_full[kRopes];
   unsigned long long done[kSlots], told[kSlots];  // the tile's MMAs are complete; its pages are known
-  unsigned long long s_full[2], s_free[2], p_full, q_full, q_free, o_full, o_free;
+  unsigned long long s_full[2], s_free[2], p_full, q_full, q_free, o_full[kOs], o_free[kOs], r_full, r_free;
   int bad[kSlots];  // of the tile's four quarters: on a page outside the cache
   int sums[kThreads / 32][2];
   Start start;
@@ -69,7 +75,7 @@ struct Smem {
 struct Args {
   CUtensorMap latent_map, rope_map;
   gemq_latent_decode_t a;
-  int* ctl;          // [0] total tiles, [1] CTAs that have some, then per entry: first tile, first row tile
+  int* ctl;          // [0] cost of the list, then per entry: where it begins in it, first row tile
   float* part_o;     // [slots][N][rank]
   float2* part_ml;   // [slots][N]: reference of the weights (in powers of two) and their sum
   int slots;
@@ -81,7 +87,7 @@ struct Args {
 __device__ __forceinline__ int start_of(const gemq_latent_decode_t& A, int g) {  // within the batch, whatever the device has
   return g <= 0 ? 0 : g >= A.groups ? A.batch : min(max(A.starts[g], 0), A.batch);
 }
-struct Entry { int len, tiles, row0, rows; };  // positions, tiles of 64, first query row (of batch * steps * heads), query rows
+struct Entry { int len, tiles, row0, rows, cost; };  // positions, tiles of 64, first query row (of batch * steps * heads), query rows; of a row tile
 
 __device__ __forceinline__ Entry entry_of(const gemq_latent_decode_t& A, int e) {
   const int per = A.steps * A.heads;
@@ -98,11 +104,15 @@ __device__ __forceinline__ Entry entry_of(const gemq_latent_decode_t& A, int e) 
     x.len = clamp_length(A.lens[b], A.table_pitch, A.page_size, A.err);
   }
   x.tiles = cdiv(x.len, kTile);
+  x.cost = x.tiles ? 4 * x.tiles + kPieceCost : 0;
   return x;
 }
-// The CTA that has a tile of the list: CTA c has tiles floor(c T / C) .. floor((c + 1) T / C) - 1.
-__device__ __forceinline__ int cta_of(long long tile, long long total, int ctas) {
-  return static_cast<int>(((tile + 1) * ctas - 1) / total);
+// Tile t of a row tile that begins at `base` of the list is at base + kPieceCost + 4 t; CTA c of C has what lies in
+// floor(c T / C) .. floor((c + 1) T / C) - 1 of the list's T.
+// A share is a tile or more: no CTA between a row tile's first and last is without one.
+__device__ __forceinline__ int ctas_of(int total, int most) { return min(most, max(total / 4, 1)); }
+__device__ __forceinline__ int cta_of(int base, int t, int total, int ctas) {
+  return static_cast<int>((static_cast<long long>(base + kPieceCost + 4 * t + 1) * ctas - 1) / total);
 }
 
 struct Piece {
@@ -110,41 +120,41 @@ struct Piece {
   int e, t0, n;      // entry, first tile, tiles
   int row0, rows;    // first query row, query rows of the row tile
   int rt;            // row tile of the launch
-  bool whole;        // all tiles of the row tile
+  __device__ __forceinline__ int width() const { return (rows + 15) & ~15; }
+  __device__ __forceinline__ bool whole() const { return n == x.tiles; }
 };
 
 template <int N>
 struct Walk {
   const gemq_latent_decode_t& A;
-  int e, rt, t, left, rto;
+  Start s;
   Entry x;
-  __device__ __forceinline__ Walk(const gemq_latent_decode_t& a, const Start& s) : A(a), e(s.e), rt(s.rt), t(s.t), left(s.left), rto(s.rto) {
-    if (left > 0) x = entry_of(A, e);
+  __device__ __forceinline__ Walk(const gemq_latent_decode_t& a, const Start& at) : A(a), s(at) {
+    if (s.from < s.to) x = entry_of(A, s.e);
   }
   __device__ __forceinline__ bool next(Piece& p) {
-    if (left <= 0) return false;
-    while (t >= x.tiles || rt * N >= x.rows) {
-      if (x.tiles > 0 && (rt + 1) * N < x.rows) {
-        ++rt;
-        t = 0;
-      } else {
-        rto += cdiv(x.rows, N);
-        rt = t = 0;
-        if (++e >= A.groups + A.batch) { left = 0; return false; }
-        x = entry_of(A, e);
+    while (s.base < s.to && s.from < s.to) {
+      if (x.cost == 0 || s.rt * N >= x.rows) {
+        s.rto += cdiv(x.rows, N);
+        s.rt = 0;
+        if (++s.e >= A.groups + A.batch) { s.to = s.from; return false; }
+        x = entry_of(A, s.e);
+        continue;
       }
+      const int t0 = min(max((s.from - s.base - kPieceCost + 3) >> 2, 0), x.tiles);
+      const int t1 = min(max((s.to - s.base - kPieceCost + 3) >> 2, 0), x.tiles);
+      p.x = x;
+      p.e = s.e;
+      p.t0 = t0;
+      p.n = t1 - t0;
+      p.row0 = x.row0 + s.rt * N;
+      p.rows = min(N, x.rows - s.rt * N);
+      p.rt = s.rto + s.rt;
+      s.base += x.cost;
+      ++s.rt;
+      if (t1 > t0) return true;
     }
-    p.x = x;
-    p.e = e;
-    p.t0 = t;
-    p.n = min(left, x.tiles - t);
-    p.row0 = x.row0 + rt * N;
-    p.rows = min(N, x.rows - rt * N);
-    p.rt = rto + rt;
-    p.whole = p.n == x.tiles;
-    t += p.n;
-    left -= p.n;
-    return true;
+    return false;
   }
 };
 
@@ -180,6 +190,20 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// Whether any of the 128 softmax threads says so; a barrier of theirs.
+__device__ __forceinline__ bool any_of_softmax(bool mine) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, 1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any)
+      : "r"(static_cast<uint32_t>(mine))
+      : "memory");
+  return any != 0;
+}
+
 template <typename T>
 __device__ __forceinline__ bool has_nonfinite(uint4 v) {
   constexpr uint32_t kExp = Pair<T>::kBf16 ? 0x7f80u : 0x7c00u;
@@ -192,28 +216,306 @@ __device__ __forceinline__ bool has_nonfinite(uint4 v) {
   return bad;
 }
 
+// ---- the softmax warps: one piece ---------------------------------------------------------------------
+template <typename T, int N, int NP>
+__device__ __forceinline__ void softmax_piece(Smem<N>& S, const Args& P, const Piece& p, uint32_t& k, uint32_t piece, uint32_t tmem,
+                                              uint32_t acc) {
+  constexpr int kLatent = Ring<N>::kLatent;
+  constexpr int kCols = NP / 4;  // rows of queries that a thread has
+  constexpr float kOffset = Pair<T>::kBf16 ? 0.f : 7.f;  // fp16 weights are 2^7 times as large: those above 2^-21 keep all their bits
+  const gemq_latent_decode_t& A = P.a;
+  int* const err = A.err;
+  const int lane = threadIdx.x & 31, quad = (threadIdx.x >> 5) & 3, blocks = A.rank / 64;
+  const bool prefix = p.e < A.groups;
+  const uint32_t lanes = static_cast<uint32_t>(32 * quad) << 16;
+  float ref[kCols], sum[kCols];  // what the weights refer to, their sums over the thread's positions
+  uint32_t none = ~0u;           // bit j: all scores of row j so far are -inf, the reference is 0
+#pragma unroll
+  for (int j = 0; j < kCols; ++j) ref[j] = sum[j] = 0.f;
+  int least = p.x.len, most = 0;
+  for (int r = lane; r < NP; r += 32) {
+    const int limit = r < p.rows ? limit_of(A, p.x, prefix, p.row0 + r) : 0;
+    if (quad == 0) S.limit[r] = limit;
+    if (r < p.rows) {
+      least = min(least, limit);
+      most = max(most, limit);
+    }
+  }
+  least = __reduce_min_sync(0xffffffffu, least);
+  most = __reduce_max_sync(0xffffffffu, most);
+  asm volatile("bar.sync 1, 128;" ::: "memory");
+  bool unset = true;
+  for (int i = 0; i < p.n; ++i, ++k) {
+    const int t0 = (p.t0 + i) * kTile;
+    wait_for(&S.told[k % kSlots], (k / kSlots) & 1, &S.abort, err);
+    const int bad = S.bad[k % kSlots];
+    wait_for(&S.s_full[k & 1], (k >> 1) & 1, &S.abort, err);
+    tc_fence_after_sync();
+    uint32_t raw[2 * kCols];
+#pragma unroll
+    for (int j = 0; j < NP / 16; ++j) tmem_load_fragments(tmem + lanes + (k & 1) * N + 16 * j, raw + 8 * j);
+    tmem_loaded(raw);
+    tc_fence_before_sync();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&S.s_free[k & 1]);
+    // v[2 j + r]: row of queries 8 (j / 2) + 2 (lane % 4) + j % 2, position 16 quad + lane / 4 + 8 r
+    float v[2 * kCols];
+#pragma unroll
+    for (int j = 0; j < kCols; ++j)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) v[2 * j + r] = fmaf(__uint_as_float(raw[4 * (j >> 1) + 2 * r + (j & 1)]), P.scale, -ref[j]);
+    const int mine = t0 + 16 * quad + (lane >> 2);
+    const bool edge = t0 + kTile > least;
+    if (edge) {
+#pragma unroll
+      for (int j = 0; j < kCols; ++j)
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+          if (mine + 8 * r >= S.limit[8 * (j >> 1) + 2 * (lane & 3) + (j & 1)]) v[2 * j + r] = -INFINITY;
+    }
+    // Weights above 2^8 times the reference move it: as a rule none, and no maximum is formed.
+    float high = v[0];
+#pragma unroll
+    for (int j = 1; j < 2 * kCols; ++j) high = fmaxf(high, v[j]);
+    const bool move = any_of_softmax(unset || high > kOffset + 8.f);
+    // the weights' place, and O, are free once the MMAs of the tile before are complete
+    if (k > 0) wait_for(&S.done[(k - 1) % kSlots], ((k - 1) / kSlots) & 1, &S.abort, err);
+    if (move) {
+      float top[kCols];
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) {
+        top[j] = fmaxf(v[2 * j], v[2 * j + 1]);
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], x));
+      }
+      if (lane < 4) {
+#pragma unroll
+        for (int j = 0; j < kCols; j += 2)
+          *reinterpret_cast<float2*>(&S.wmax[quad][4 * j + 2 * lane]) = make_float2(top[j], top[j + 1]);
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      float f[kCols];
+      unset = false;
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) {
+        const int col = 8 * (j >> 1) + 2 * (lane & 3) + (j & 1);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) top[j] = fmaxf(top[j], S.wmax[w][col]);
+        // relative to the reference so far; a row that has none takes what there is
+        const bool new_one = none >> j & 1;
+        const float up = new_one ? top[j] - kOffset : fmaxf(top[j] - kOffset, 0.f);
+        const bool still = up == -INFINITY;
+        const float by = still ? 0.f : up;
+        if (!still) none &= ~(1u << j);
+        unset |= still && S.limit[col] > 0;
+        f[j] = new_one ? 1.f : exp2_fast(-by);
+        ref[j] += by;
+        sum[j] *= f[j];
+        v[2 * j] -= by;
+        v[2 * j + 1] -= by;
+      }
+      unset = __any_sync(0xffffffffu, unset);
+      if (i > 0) {
+        if (lane < 4 && quad == 0) {
+#pragma unroll
+          for (int j = 0; j < kCols; j += 2) *reinterpret_cast<float2*>(&S.fac[4 * j + 2 * lane]) = make_float2(f[j], f[j + 1]);
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        tc_fence_after_sync();
+        for (int m = 0; m < blocks / 2; ++m)
+#pragma unroll
+          for (int j = 0; j < NP; j += 16) {
+            uint32_t o[16];
+            tmem_load16(acc + lanes + m * N + j, o);
+            tmem_loaded(o);
+#pragma unroll
+            for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * S.fac[j + x]);
+            tmem_store16(acc + lanes + m * N + j, o);
+          }
+        tmem_stored();
+        tc_fence_before_sync();
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 2 * kCols; ++j) v[j] = exp2_fast(v[j]);
+    // Rows of the tile that not all queries see: nothing of them may come through a weight of 0.  A page that is none: NaN.
+    if (edge || bad) {
+      uint32_t poison = 0;
+      if (edge) {
+        const int block = static_cast<int>(k) * blocks + (lane >> 2);  // lane: 32 bytes of one of the rank's blocks
+        for (int d = 0; d < blocks; d += 2) {  // complete, as S is: that this thread sees what TMA wrote
+          const int q = static_cast<int>(k) * blocks + d;
+          wait_for(&S.full[q % kLatent / 2], (q / kLatent) & 1, &S.abort, err);
+        }
+        for (int r = max(least - t0 - 16 * quad, 0); r < 16; ++r) {
+          const int pos = t0 + 16 * quad + r;
+          uint4* at = reinterpret_cast<uint4*>(S.ring[block % kLatent] + (16 * quad + r) * 128) + 2 * (lane & 3);
+          const bool have = (lane >> 2) < blocks;
+          bool wipe = pos >= most;
+          if (!wipe) {
+            wipe = __any_sync(0xffffffffu, have && (has_nonfinite<T>(at[0]) || has_nonfinite<T>(at[1])));
+            if (wipe) poison |= 1u << r;
+          }
+          if (wipe && have) at[0] = at[1] = make_uint4(0, 0, 0, 0);
+        }
+      }
+      if (bad >> quad & 1) poison = 0xffff;
+#pragma unroll
+      for (int j = 0; j < kCols; ++j)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          if (poison >> ((lane >> 2) + 8 * r) & 1) v[2 * j + r] = __int_as_float(0x7fc00000);
+          if (mine + 8 * r >= S.limit[8 * (j >> 1) + 2 * (lane & 3) + (j & 1)]) v[2 * j + r] = 0.f;
+        }
+    }
+    uint32_t w[kCols];
+#pragma unroll
+    for (int j = 0; j < kCols; ++j) sum[j] += v[2 * j] + v[2 * j + 1];
+#pragma unroll
+    for (int j = 0; j < kCols; j += 2) {
+      w[j] = Pair<T>::r(v[2 * j], v[2 * j + 2]);          // position lane / 4
+      w[j + 1] = Pair<T>::r(v[2 * j + 1], v[2 * j + 3]);  // ... + 8
+    }
+    // transposed 8 x 8 blocks: a row of queries has its 64 weights in 128 bytes, 16-byte pieces swizzled by the row
+#pragma unroll
+    for (int j = 0; j < NP / 16; ++j) {
+      const int row = 16 * j + 8 * (lane >> 4) + (lane & 7), piece16 = 2 * quad + ((lane >> 3) & 1);
+      asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(
+                       smem_u32(S.p) + row * 128 + ((piece16 ^ (row & 7)) << 4)),
+                   "r"(w[4 * j]), "r"(w[4 * j + 1]), "r"(w[4 * j + 2]), "r"(w[4 * j + 3])
+                   : "memory");
+    }
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&S.p_full);
+  }
+  // sums of the weights over the positions
+#pragma unroll
+  for (int j = 0; j < kCols; ++j)
+#pragma unroll
+    for (int x = 4; x < 32; x <<= 1) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], x);
+  asm volatile("bar.sync 1, 128;" ::: "memory");  // maxima and factors of the last correction are read
+  if (lane < 4) {
+#pragma unroll
+    for (int j = 0; j < kCols; j += 2) {
+      *reinterpret_cast<float2*>(&S.wmax[quad][4 * j + 2 * lane]) = make_float2(sum[j], sum[j + 1]);
+      if (quad == 0)
+        *reinterpret_cast<float2*>(&S.fac[4 * j + 2 * lane]) =
+            make_float2(none >> j & 1 ? -INFINITY : ref[j], none >> (j + 1) & 1 ? -INFINITY : ref[j + 1]);
+    }
+  }
+  wait_for(&S.r_free, (piece & 1) ^ 1, &S.abort, err);
+  asm volatile("bar.sync 1, 128;" ::: "memory");
+  const int me = 32 * quad + lane;
+  if (me < NP) S.result[me] = make_float2(S.fac[me], S.wmax[0][me] + S.wmax[1][me] + S.wmax[2][me] + S.wmax[3][me]);
+  __syncwarp();
+  if (lane == 0) mbar_arrive(&S.r_full);
+}
+
+// ---- the warps at a piece's two ends ------------------------------------------------------------------
+// Its queries: eight lanes a row's 128 bytes of a block.
+template <typename T, int N>
+__device__ __forceinline__ void load_queries(Smem<N>& S, const gemq_latent_decode_t& A, const Piece& p, uint32_t piece) {
+  const int tid = static_cast<int>(threadIdx.x) - 32 * kEdgeWarp, per = A.steps * A.heads, blocks = A.rank / 64, chunks = A.rank / 8 + 8;
+  wait_for(&S.q_free, (piece & 1) ^ 1, &S.abort, A.err);
+  for (int r = tid >> 3; r < p.width(); r += 16) {
+    const int row = p.row0 + r, b = row / per, i = row % per / A.heads, h = row % A.heads;
+    const bool on = r < p.rows;
+    const uint4* ql = reinterpret_cast<const uint4*>(static_cast<const T*>(A.q_latent) + b * A.q_latent_stride[0] + i * A.q_latent_stride[1] +
+                                                     h * A.q_latent_stride[2]);
+    const uint4* qr = reinterpret_cast<const uint4*>(static_cast<const T*>(A.q_rope) + b * A.q_rope_stride[0] + i * A.q_rope_stride[1] +
+                                                     h * A.q_rope_stride[2]);
+    uint4 v[9];
+#pragma unroll
+    for (int d = 0; d < 9; ++d) {
+      const int at = d * 8 + (tid & 7);
+      v[d] = make_uint4(0, 0, 0, 0);
+      if (on && at < chunks) v[d] = at < chunks - 8 ? ql[at] : qr[at - (chunks - 8)];
+    }
+#pragma unroll
+    for (int d = 0; d < 9; ++d)
+      if (d <= blocks) *reinterpret_cast<uint4*>(S.q[d] + r * 128 + (((tid & 7) ^ (r & 7)) << 4)) = v[d];
+  }
+  fence_async_smem();
+  __syncwarp();
+  if ((tid & 31) == 0) mbar_arrive(&S.q_full);
+}
+
+// Its results: thread 32 quad + lane has dimension 128 m + that of all rows of queries.
+template <typename T, int N>
+__device__ __forceinline__ void finish_piece(Smem<N>& S, const Args& P, const Piece& p, uint32_t piece, uint32_t acc) {
+  constexpr int kOs = Smem<N>::kOs;
+  const gemq_latent_decode_t& A = P.a;
+  const int lane = threadIdx.x & 31, quad = (threadIdx.x >> 5) & 3, me = 32 * quad + lane;
+  const uint32_t lanes = static_cast<uint32_t>(32 * quad) << 16;
+  const bool prefix = p.e < A.groups, whole = p.whole() && A.groups == 0;
+  const int slot = p.rt + static_cast<int>(blockIdx.x);  // pieces of the launch in order: either grows
+  if (slot >= P.slots) atomicExch(A.err, GEMQ_LATENT_BAD_LENGTH);
+  wait_for(&S.r_full, piece & 1, &S.abort, A.err);
+  if (me < p.rows && (whole || slot < P.slots)) {
+    const float2 r = S.result[me];
+    if (whole) A.lse[p.row0 + me] = limit_of(A, p.x, prefix, p.row0 + me) > 0 ? (r.x + log2f(r.y)) * kLn2 : -INFINITY;
+    else P.part_ml[static_cast<long long>(slot) * N + me] = r;
+  }
+  wait_for(&S.o_full[piece % kOs], (piece / kOs) & 1, &S.abort, A.err);
+  tc_fence_after_sync();
+  for (int m = 0; m < A.rank / 128; ++m)
+#pragma unroll 1
+    for (int j = 0; j < p.rows; j += 16) {
+      uint32_t o[16];
+      tmem_load16(acc + lanes + m * N + j, o);
+      tmem_loaded(o);
+      if (whole) {
+        T* out = static_cast<T*>(A.out) + static_cast<long long>(p.row0 + j) * A.rank + 128 * m + (me & ~1);
+#pragma unroll
+        for (int x = 0; x < 16; x += 2) {  // an even lane takes row x of a pair of dimensions, its neighbour row x + 1
+          const float give = __uint_as_float(lane & 1 ? o[x] : o[x + 1]), keep = __uint_as_float(lane & 1 ? o[x + 1] : o[x]);
+          const float got = __shfl_xor_sync(0xffffffffu, give, 1);
+          const int r = x + (lane & 1), col = j + r;
+          if (col < p.rows) {
+            const float l = S.result[col].y;
+            const float f = l == 0.f && limit_of(A, p.x, prefix, p.row0 + col) <= 0 ? 0.f : 1.f / l;
+            *reinterpret_cast<uint32_t*>(out + r * static_cast<long long>(A.rank)) =
+                lane & 1 ? Pair<T>::r(got * f, keep * f) : Pair<T>::r(keep * f, got * f);
+          }
+        }
+      } else if (slot < P.slots) {
+        float* out = P.part_o + (static_cast<long long>(slot) * N + j) * A.rank + 128 * m + me;
+#pragma unroll
+        for (int x = 0; x < 16; ++x)
+          if (j + x < p.rows) out[x * static_cast<long long>(A.rank)] = __uint_as_float(o[x]);
+      }
+    }
+  tc_fence_before_sync();
+  __syncwarp();
+  if (lane == 0) {
+    mbar_arrive(&S.r_free);
+    mbar_arrive(&S.o_free[piece % kOs]);
+  }
+}
+
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid_constant__ Args P) {
   constexpr int kLatent = Ring<N>::kLatent, kRopes = Ring<N>::kRopes;
-  constexpr uint32_t kTmemCols = N == 16 ? 128 : N == 32 ? 256 : 512;
+  constexpr uint32_t kTmemCols = N == 16 ? 256 : 512;
   constexpr uint32_t kTmemO = 2 * N;
-  constexpr int kCols = N / 4;  // rows of queries that a softmax thread has
-  constexpr float kOffset = Pair<T>::kBf16 ? 0.f : 7.f;  // fp16 weights are 2^7 times as large: those above 2^-21 keep all their bits
+  constexpr int kOs = Smem<N>::kOs;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   Smem<N>& S = *reinterpret_cast<Smem<N>*>(smem_raw);
   const gemq_latent_decode_t& A = P.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int blocks = A.rank / 64;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kLatent / 2; ++i) mbar_init(&S.full[i], 1);
+    for (int i = 0; i < kLatent / 2; ++i) { mbar_init(&S.full[i], 1); mbar_init(&S.empty[i], 1); }
     for (int i = 0; i < kRopes; ++i) mbar_init(&S.rope_full[i], 1);
     for (int i = 0; i < kSlots; ++i) { mbar_init(&S.done[i], 1); mbar_init(&S.told[i], 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(&S.s_full[i], 1); mbar_init(&S.s_free[i], 4); }
     mbar_init(&S.p_full, 4);
-    mbar_init(&S.q_full, 2);
+    mbar_init(&S.q_full, 4);
     mbar_init(&S.q_free, 1);
-    mbar_init(&S.o_full, 1);
-    mbar_init(&S.o_free, 4);
+    for (int i = 0; i < kOs; ++i) { mbar_init(&S.o_full[i], 1); mbar_init(&S.o_free[i], 4); }
+    mbar_init(&S.r_full, 4);
+    mbar_init(&S.r_free, 4);
     S.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -222,16 +524,16 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
 
   // Every CTA adds up the list: a thread has a run of entries.
   const int entries = A.groups + A.batch, run = cdiv(entries, kThreads);
-  int tiles = 0, rts = 0;
+  int cost = 0, rts = 0;
   for (int k = 0; k < run; ++k) {
     const int e = static_cast<int>(threadIdx.x) * run + k;
     if (e >= entries) break;
     const Entry x = entry_of(A, e);
     const int n = cdiv(x.rows, N);
-    tiles += n * x.tiles;
+    cost += n * x.cost;
     rts += n;
   }
-  int before = tiles, rts_before = rts;
+  int before = cost, rts_before = rts;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
     const int a = __shfl_up_sync(0xffffffffu, before, d), b = __shfl_up_sync(0xffffffffu, rts_before, d);
@@ -243,7 +545,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
   tc_fence_after_sync();
   // Only now: a CTA of the next kernel must not take this SM's tensor memory first.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  before -= tiles;
+  before -= cost;
   rts_before -= rts;
   int total = 0;
 #pragma unroll
@@ -251,86 +553,102 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     if (w < warp) { before += S.sums[w][0]; rts_before += S.sums[w][1]; }
     total += S.sums[w][0];
   }
-  const int ctas = min(static_cast<int>(gridDim.x), total), c = blockIdx.x;
-  const int first = c < ctas ? static_cast<int>(static_cast<long long>(c) * total / ctas) : 0;
-  const int last = c < ctas ? static_cast<int>(static_cast<long long>(c + 1) * total / ctas) : 0;
+  const int ctas = ctas_of(total, gridDim.x), c = blockIdx.x;
+  const int from = c < ctas ? static_cast<int>(static_cast<long long>(c) * total / ctas) : 0;
+  const int to = c < ctas ? static_cast<int>(static_cast<long long>(c + 1) * total / ctas) : 0;
   if (c == 0 && threadIdx.x == 0) {
     P.ctl[0] = total;
-    P.ctl[1] = ctas;
     if (A.groups > 0 && !offsets_ok(A.starts, A.groups, A.batch, true)) atomicExch(A.err, GEMQ_LATENT_BAD_LENGTH);
   }
-  if (c == 0 || (c < ctas && first >= before && first < before + tiles)) {
+  if (c == 0 || (from >= before && from < before + cost)) {
     int at = before, rto = rts_before;
     for (int k = 0; k < run; ++k) {
       const int e = static_cast<int>(threadIdx.x) * run + k;
       if (e >= entries) break;
       const Entry x = entry_of(A, e);
-      const int n = cdiv(x.rows, N), all = n * x.tiles;
+      const int n = cdiv(x.rows, N), all = n * x.cost;
       if (c == 0) {
         P.ctl[2 + 2 * e] = at;
         P.ctl[3 + 2 * e] = rto;
       }
-      if (c < ctas && first >= at && first < at + all) S.start = {e, (first - at) / x.tiles, (first - at) % x.tiles, last - first, rto};
+      if (from >= at && from < at + all) {
+        const int rt = (from - at) / x.cost;
+        S.start = {e, rt, at + rt * x.cost, from, to, rto};
+      }
       at += all;
       rto += n;
     }
   }
   __syncthreads();
   const uint32_t tmem = S.tmem_base;
-  const Start start = c < ctas ? S.start : Start{0, 0, 0, 0, 0};
+  const Start start = from < to ? S.start : Start{0, 0, 0, 0, 0, 0};
   int* const err = A.err;
-
+  // 64 rows of queries: 240 registers for the softmax warps; with the others' 88 and 168 below the launch's 3 x 168
+  if (warp < kSoftWarp) {
+  if (N == 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   if (warp == 0) {
     Walk<N> walk(A, start);
     Piece p;
-    int block = 0, freed = 0;      // latent blocks asked for so far; tiles known to be done
-    uint32_t k = 0;
-    const int per_tile = A.page_size < kTile ? kTile / A.page_size : 1, quarters = A.page_size < kTile ? A.page_size / 16 : 4;
-    const int box_rows = min(A.page_size, kTile);
+    int place = 0, freed = 0;  // next latent block of the ring; tiles known to be done
+    uint32_t k = 0, phase = 1;
+    const bool small = A.page_size < kTile;
+    const int per_tile = small ? kTile / A.page_size : 1, quarters = small ? A.page_size / 16 : 4, tiles_a_page = small ? 1 : A.page_size / kTile;
+    const int box_rows = min(A.page_size, kTile), boxes = 2 / P.box_blocks;
     while (walk.next(p)) {
       const bool prefix = p.e < A.groups;
       const int* table = prefix ? A.prefix_table + static_cast<long long>(p.e) * A.prefix_pitch
                                 : A.table + static_cast<long long>(p.e - A.groups) * A.table_pitch;
       const int pages = (p.x.len + A.page_size - 1) / A.page_size;
-      int base = -64, ids = 0;     // lane i has the id of page base + i
-      for (int t = p.t0; t < p.t0 + p.n; ++t, ++k) {
-        const int pg = A.page_size < kTile ? t * per_tile : t * kTile / A.page_size;
+      int pg = small ? p.t0 * per_tile : p.t0 / tiles_a_page, row = small ? 0 : (p.t0 % tiles_a_page) * kTile;
+      int base = pg, ids = base + lane < pages ? table[base + lane] : 0;  // lane i has the id of page base + i
+      for (int i = 0; i < p.n; ++i, ++k) {
         const int here = min(per_tile, pages - pg);  // pages of the tile
-        if (pg < base || pg + here > base + 32) {
+        if (pg + here > base + 32) {
           base = pg;
           ids = base + lane < pages ? table[base + lane] : 0;
         }
         const bool out = (ids < 0 || ids >= A.n_pages) && base + lane < pages;
         const uint32_t outs = __ballot_sync(0xffffffffu, out) >> (pg - base);
         int bad = 0;
-        for (int i = 0; i < here; ++i)
-          if ((outs >> i) & 1) bad |= ((1 << quarters) - 1) << (i * quarters);
+        for (int j = 0; j < here; ++j)
+          if ((outs >> j) & 1) bad |= ((1 << quarters) - 1) << (j * quarters);
         if (lane == 0) {
           S.bad[k % kSlots] = bad;
           mbar_arrive(&S.told[k % kSlots]);
           if (bad) atomicExch(err, GEMQ_LATENT_BAD_PAGE);
         }
-        const int row = A.page_size < kTile ? 0 : t * kTile % A.page_size;
         const uint32_t bytes = here * box_rows * 128;
-        // Block q of the ring was block q - kLatent, of tile (q - kLatent) / blocks.
-        for (int d = 0; d <= blocks; d += 2) {
-          const bool rope = d == blocks;
-          const int need = rope ? static_cast<int>(k) - kRopes + 1 : (block + 1 - kLatent) / blocks + (block + 1 >= kLatent ? 1 : 0);
-          for (; freed < need; ++freed) wait_for(&S.done[freed % kSlots], (freed / kSlots) & 1, &S.abort, err);
-          unsigned char* dst = rope ? S.rope[k % kRopes] : S.ring[block % kLatent];
-          unsigned long long* bar = rope ? &S.rope_full[k % kRopes] : &S.full[block % kLatent / 2];
-          if (lane == 0) mbar_arrive_expect_tx(bar, rope ? bytes : 2 * bytes);
-          __syncwarp();
-          const int boxes = rope ? 1 : 2 / P.box_blocks;
-          for (int i = 0; i < here; ++i) {
-            const int id = __shfl_sync(0xffffffffu, out ? 0 : ids, pg - base + i);
-            if (elect_lane()) {
-              for (int j = 0; j < boxes; ++j)
-                tma_load_4d(dst + j * kBlock + i * A.page_size * 128, rope ? &P.rope_map : &P.latent_map, 0, row, d + j, id, bar);
-            }
-            __syncwarp();
+        int id[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) id[j] = __shfl_sync(0xffffffffu, out ? 0 : ids, (pg - base + j) & 31);
+        for (int d = 0; d < blocks; d += 2) {
+          wait_for(&S.empty[place >> 1], phase, &S.abort, err);
+          unsigned char* dst = S.ring[place];
+          unsigned long long* bar = &S.full[place >> 1];
+          if (elect_lane()) {
+            mbar_arrive_expect_tx(bar, 2 * bytes);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (j < here)
+                for (int n = 0; n < boxes; ++n) tma_load_4d(dst + n * kBlock + j * A.page_size * 128, &P.latent_map, 0, row, d + n, id[j], bar);
           }
-          if (!rope) block += 2;
+          __syncwarp();
+          place += 2;
+          if (place == kLatent) { place = 0; phase ^= 1; }
+        }
+        for (; static_cast<int>(k) >= kRopes + freed; ++freed) wait_for(&S.done[freed % kSlots], (freed / kSlots) & 1, &S.abort, err);
+        if (elect_lane()) {
+          mbar_arrive_expect_tx(&S.rope_full[k % kRopes], bytes);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (j < here) tma_load_4d(S.rope[k % kRopes] + j * A.page_size * 128, &P.rope_map, 0, row, blocks, id[j], &S.rope_full[k % kRopes]);
+        }
+        __syncwarp();
+        if (small) {
+          pg += per_tile;
+        } else {
+          row += kTile;
+          if (row == A.page_size) { row = 0; ++pg; }
         }
       }
     }
@@ -338,320 +656,104 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     if (*reinterpret_cast<volatile int*>(&S.abort))
       for (int i = 0; i < 2000; ++i) __nanosleep(1000);
   } else if (warp == 1) {
+    // The whole warp runs the loop and one elected lane issues: descriptors stay in uniform registers.
     Walk<N> walk(A, start);
     Piece p;
-    uint32_t k = 0, piece = 0;
-    const uint32_t idesc_s = umma_idesc_f16(Pair<T>::kBf16, kTile, N), idesc_o = umma_idesc_f16(Pair<T>::kBf16, 128, N) | kUmmaTransposeA;
-    const uint64_t q0 = umma_desc_k_sw128(smem_u32(S.q[0])), p0 = umma_desc_k_sw128(smem_u32(S.p));
-    const uint32_t ring0 = smem_u32(S.ring[0]);
-    // O of a tile: its place in the ring, 16-row steps, whether it is the piece's first and last
-    int prev_block = -1, prev_steps = 0;
-    bool prev_first = false, prev_last = false;
-    uint32_t prev_k = 0, prev_piece = 0;
-    auto values = [&]() {
-      if (prev_first) wait_for(&S.o_free, (prev_piece & 1) ^ 1, &S.abort, err);
-      wait_for(&S.p_full, prev_k & 1, &S.abort, err);
-      tc_fence_after_sync();
-      if (elect_lane()) {
-        int at = prev_block % kLatent;
-        for (int m = 0; m < blocks / 2; ++m) {
-          const uint64_t a = umma_desc_mn_sw128(ring0 + at * kBlock, kBlock);
-          for (int s = 0; s < prev_steps; ++s)
-            umma_ss_f16(tmem + kTmemO + m * N, a + s * (2048 >> 4), p0 + s * (32 >> 4), idesc_o, !prev_first || s != 0);
-          at = at + 2 == kLatent ? 0 : at + 2;
-        }
-        umma_commit(&S.done[prev_k % kSlots]);
-        if (prev_last) umma_commit(&S.o_full);
-      }
-      __syncwarp();
-    };
-    int block = 0;
-    while (walk.next(p)) {
-      for (int i = 0; i < p.n; ++i, ++k, block += blocks) {
-        if (i == 0) wait_for(&S.q_full, piece & 1, &S.abort, err);
+    const uint64_t q0 = umma_desc_k_sw128(smem_u32(S.q[0])), ring0 = umma_desc_k_sw128(smem_u32(S.ring[0])),
+                   rope0 = umma_desc_k_sw128(smem_u32(S.rope[0]));
+    uint32_t k = 0, phase = 0, rope_at = 0, rope_phase = 0;
+    int place = 0;
+    for (uint32_t piece = 0; walk.next(p); ++piece) {
+      const uint32_t idesc = umma_idesc_f16(Pair<T>::kBf16, kTile, p.width());
+      wait_for(&S.q_full, piece & 1, &S.abort, err);
+      for (int i = 0; i < p.n; ++i, ++k) {
         wait_for(&S.s_free[k & 1], ((k >> 1) & 1) ^ 1, &S.abort, err);
-        tc_fence_after_sync();
         const uint32_t s = tmem + (k & 1) * N;
-        for (int d = 0; d <= blocks; ++d) {
-          const bool rope = d == blocks;
-          const int q = block + d;
-          if (rope) wait_for(&S.rope_full[k % kRopes], (k / kRopes) & 1, &S.abort, err);
-          else if (!(d & 1)) wait_for(&S.full[q % kLatent / 2], (q / kLatent) & 1, &S.abort, err);
+        for (int d = 0; d < blocks; d += 2) {
+          wait_for(&S.full[place >> 1], phase, &S.abort, err);
+          tc_fence_after_sync();
+          const uint64_t a = ring0 + place * (kBlock >> 4), b = q0 + d * (N * 128 >> 4);
           if (elect_lane()) {
-            const uint64_t a = umma_desc_k_sw128(rope ? smem_u32(S.rope[k % kRopes]) : ring0 + q % kLatent * kBlock);
-            const uint64_t b = q0 + d * (N * 128 >> 4);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) umma_ss_f16(s, a + j * 2, b + j * 2, idesc_s, d != 0 || j != 0);
+            for (int j = 0; j < 8; ++j)
+              umma_ss_f16(s, a + (j >> 2) * (kBlock >> 4) + (j & 3) * 2, b + (j >> 2) * (N * 128 >> 4) + (j & 3) * 2, idesc, d != 0 || j != 0);
           }
           __syncwarp();
+          place += 2;
+          if (place == kLatent) { place = 0; phase ^= 1; }
         }
+        wait_for(&S.rope_full[rope_at], rope_phase, &S.abort, err);
+        tc_fence_after_sync();
+        const uint64_t a = rope0 + rope_at * (kBlock >> 4), b = q0 + blocks * (N * 128 >> 4);
         if (elect_lane()) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) umma_ss_f16(s, a + j * 2, b + j * 2, idesc, 1);
           umma_commit(&S.s_full[k & 1]);
           if (i == p.n - 1) umma_commit(&S.q_free);
         }
         __syncwarp();
-        if (prev_block >= 0) values();
-        prev_block = block;
-        prev_k = k;
-        prev_piece = piece;
-        prev_first = i == 0;
-        prev_last = i == p.n - 1;
-        prev_steps = cdiv(min(p.x.len - (p.t0 + i) * kTile, kTile), 16);
+        if (++rope_at == kRopes) { rope_at = 0; rope_phase ^= 1; }
       }
-      ++piece;
     }
-    if (prev_block >= 0) values();
-  } else if (warp < kSoftWarp) {
+  } else if (warp == 2) {
     Walk<N> walk(A, start);
     Piece p;
-    const int tid = static_cast<int>(threadIdx.x) - 64, per = A.steps * A.heads, chunks = A.rank / 8 + 8;
+    const uint64_t p0 = umma_desc_k_sw128(smem_u32(S.p)), ring0 = umma_desc_mn_sw128(smem_u32(S.ring[0]), kBlock);
+    uint32_t k = 0;
+    int place = 0;
     for (uint32_t piece = 0; walk.next(p); ++piece) {
-      wait_for(&S.q_free, (piece & 1) ^ 1, &S.abort, err);
-      // eight lanes a row's 128 bytes
-      for (int r = tid >> 3; r < N; r += 8) {
-        const int row = p.row0 + r, b = row / per, i = row % per / A.heads, h = row % A.heads;
-        const bool on = r < p.rows;
-        const uint4* ql = reinterpret_cast<const uint4*>(static_cast<const T*>(A.q_latent) + b * A.q_latent_stride[0] + i * A.q_latent_stride[1] +
-                                                         h * A.q_latent_stride[2]);
-        const uint4* qr = reinterpret_cast<const uint4*>(static_cast<const T*>(A.q_rope) + b * A.q_rope_stride[0] + i * A.q_rope_stride[1] +
-                                                         h * A.q_rope_stride[2]);
-        uint4 v[9];
+      const uint32_t idesc = umma_idesc_f16(Pair<T>::kBf16, 128, p.width()) | kUmmaTransposeA;
+      const uint32_t acc = tmem + kTmemO + piece % kOs * (4 * N);
+      wait_for(&S.o_free[piece % kOs], ((piece / kOs) & 1) ^ 1, &S.abort, err);
+      for (int i = 0; i < p.n; ++i, ++k) {
+        const int steps = cdiv(min(p.x.len - (p.t0 + i) * kTile, kTile), 16);  // of 16 positions
+        wait_for(&S.p_full, k & 1, &S.abort, err);
+        tc_fence_after_sync();
+        // a pair of blocks is free behind its MMAs: S of the tile is complete
+        for (int m = 0; m < blocks / 2; ++m) {
+          const uint64_t a = ring0 + place * (kBlock >> 4);
+          const uint32_t o = acc + m * N;
+          if (elect_lane()) {
+            umma_ss_f16(o, a, p0, idesc, i != 0);
+            if (steps == 4) {
 #pragma unroll
-        for (int d = 0; d < 9; ++d) {
-          const int at = d * 8 + (tid & 7);
-          v[d] = make_uint4(0, 0, 0, 0);
-          if (on && at < chunks) v[d] = at < chunks - 8 ? ql[at] : qr[at - (chunks - 8)];
+              for (int s = 1; s < 4; ++s) umma_ss_f16(o, a + s * (2048 >> 4), p0 + s * (32 >> 4), idesc, 1);
+            } else {
+              for (int s = 1; s < steps; ++s) umma_ss_f16(o, a + s * (2048 >> 4), p0 + s * (32 >> 4), idesc, 1);
+            }
+            umma_commit(&S.empty[place >> 1]);
+          }
+          __syncwarp();
+          place = place + 2 == kLatent ? 0 : place + 2;
         }
-#pragma unroll
-        for (int d = 0; d < 9; ++d)
-          if (d <= blocks) *reinterpret_cast<uint4*>(S.q[d] + r * 128 + (((tid & 7) ^ (r & 7)) << 4)) = v[d];
+        if (elect_lane()) {
+          umma_commit(&S.done[k % kSlots]);
+          if (i == p.n - 1) umma_commit(&S.o_full[piece % kOs]);
+        }
+        __syncwarp();
       }
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&S.q_full);
+    }
+  }
+  } else if (warp >= kEdgeWarp) {
+    Walk<N> ahead(A, start), walk(A, start);
+    Piece q, p;
+    uint32_t loads = 0;
+    if (ahead.next(q)) load_queries<T, N>(S, A, q, loads++);
+    for (uint32_t piece = 0; walk.next(p); ++piece) {
+      if (ahead.next(q)) load_queries<T, N>(S, A, q, loads++);
+      finish_piece<T, N>(S, P, p, piece, tmem + kTmemO + piece % kOs * (4 * N));
     }
   } else {
+    if (N == 64) asm volatile("setmaxnreg.inc.sync.aligned.u32 240;");
     Walk<N> walk(A, start);
     Piece p;
-    const int quad = warp & 3;
-    const uint32_t lanes = static_cast<uint32_t>(32 * quad) << 16;
     uint32_t k = 0;
     for (uint32_t piece = 0; walk.next(p); ++piece) {
-      const bool prefix = p.e < A.groups;
-      float ref[kCols], sum[kCols];
-      int limit[kCols], least = p.x.len, most = 0;
-#pragma unroll
-      for (int j = 0; j < kCols; ++j) {
-        const int col = 8 * (j >> 1) + 2 * (lane & 3) + (j & 1);
-        ref[j] = -INFINITY;
-        sum[j] = 0.f;
-        limit[j] = 0;
-        if (col < p.rows) {
-          limit[j] = limit_of(A, p.x, prefix, p.row0 + col);
-          least = min(least, limit[j]);
-          most = max(most, limit[j]);
-        }
-      }
-#pragma unroll
-      for (int x = 1; x < 4; x <<= 1) {
-        least = min(least, __shfl_xor_sync(0xffffffffu, least, x));
-        most = max(most, __shfl_xor_sync(0xffffffffu, most, x));
-      }
-      for (int i = 0; i < p.n; ++i, ++k) {
-        const int t0 = (p.t0 + i) * kTile;
-        wait_for(&S.told[k % kSlots], (k / kSlots) & 1, &S.abort, err);
-        const int bad = S.bad[k % kSlots];
-        wait_for(&S.s_full[k & 1], (k >> 1) & 1, &S.abort, err);
-        tc_fence_after_sync();
-        uint32_t raw[2 * kCols];
-#pragma unroll
-        for (int j = 0; j < N / 16; ++j) tmem_load_fragments(tmem + lanes + (k & 1) * N + 16 * j, raw + 8 * j);
-        tmem_loaded(raw);
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&S.s_free[k & 1]);
-        // v[2 j + r]: row of queries 8 (j / 2) + 2 (lane % 4) + j % 2, position 16 quad + lane / 4 + 8 r
-        float v[2 * kCols];
-#pragma unroll
-        for (int j = 0; j < kCols; ++j)
-#pragma unroll
-          for (int r = 0; r < 2; ++r) v[2 * j + r] = __uint_as_float(raw[4 * (j >> 1) + 2 * r + (j & 1)]) * P.scale;
-        const int mine = t0 + 16 * quad + (lane >> 2);
-        const bool edge = t0 + kTile > least;
-        if (edge) {
-#pragma unroll
-          for (int j = 0; j < kCols; ++j)
-#pragma unroll
-            for (int r = 0; r < 2; ++r)
-              if (mine + 8 * r >= limit[j]) v[2 * j + r] = -INFINITY;
-        }
-        float top[kCols];
-#pragma unroll
-        for (int j = 0; j < kCols; ++j) {
-          top[j] = fmaxf(v[2 * j], v[2 * j + 1]);
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], x));
-        }
-        if (lane < 4) {
-#pragma unroll
-          for (int j = 0; j < kCols; j += 2)
-            *reinterpret_cast<float2*>(&S.wmax[k & 1][quad][4 * j + 2 * lane]) = make_float2(top[j], top[j + 1]);
-        }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-#pragma unroll
-          for (int j = 0; j < kCols; j += 2) {
-            const float2 f = *reinterpret_cast<const float2*>(&S.wmax[k & 1][w][4 * j + 2 * (lane & 3)]);
-            top[j] = fmaxf(top[j], f.x);
-            top[j + 1] = fmaxf(top[j + 1], f.y);
-          }
-        bool move = false;
-#pragma unroll
-        for (int j = 0; j < kCols; ++j) move |= top[j] > ref[j] + (kOffset + 8.f);
-        // the weights' place, and O, are free once the MMAs of the tile before are complete
-        if (i > 0) wait_for(&S.done[(k - 1) % kSlots], ((k - 1) / kSlots) & 1, &S.abort, err);
-        if (__any_sync(0xffffffffu, move)) {  // the same in all four warps
-          float f[kCols];
-#pragma unroll
-          for (int j = 0; j < kCols; ++j) {
-            const float now = fmaxf(ref[j], top[j] - kOffset);
-            f[j] = now == -INFINITY ? 1.f : exp2_fast(ref[j] - now);
-            ref[j] = now;
-            sum[j] *= f[j];
-          }
-          if (i > 0) {
-            if (lane < 4 && quad == 0) {
-#pragma unroll
-              for (int j = 0; j < kCols; j += 2) *reinterpret_cast<float2*>(&S.fac[4 * j + 2 * lane]) = make_float2(f[j], f[j + 1]);
-            }
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            tc_fence_after_sync();
-            for (int m = 0; m < blocks / 2; ++m)
-#pragma unroll
-              for (int j = 0; j < N; j += 16) {
-                uint32_t o[16];
-                tmem_load16(tmem + lanes + kTmemO + m * N + j, o);
-                tmem_loaded(o);
-#pragma unroll
-                for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * S.fac[j + x]);
-                tmem_store16(tmem + lanes + kTmemO + m * N + j, o);
-              }
-            tmem_stored();
-            tc_fence_before_sync();
-          }
-        }
-        // Rows of the tile that not all queries see: nothing of them may come through a weight of 0.
-        uint32_t poison = 0;
-        if (edge) {
-          const int block = static_cast<int>(k) * blocks + (lane >> 2);  // lane: 32 bytes of one of the rank's blocks
-          for (int d = 0; d < blocks; d += 2) {  // complete, as S is: that this thread sees what TMA wrote
-            const int q = static_cast<int>(k) * blocks + d;
-            wait_for(&S.full[q % kLatent / 2], (q / kLatent) & 1, &S.abort, err);
-          }
-          for (int r = max(least - t0 - 16 * quad, 0); r < 16; ++r) {
-            const int pos = t0 + 16 * quad + r;
-            uint4* at = reinterpret_cast<uint4*>(S.ring[block % kLatent] + (16 * quad + r) * 128) + 2 * (lane & 3);
-            const bool have = (lane >> 2) < blocks;
-            bool wipe = pos >= most;
-            if (!wipe) {
-              wipe = __any_sync(0xffffffffu, have && (has_nonfinite<T>(at[0]) || has_nonfinite<T>(at[1])));
-              if (wipe) poison |= 1u << r;
-            }
-            if (wipe && have) at[0] = at[1] = make_uint4(0, 0, 0, 0);
-          }
-        }
-        if (bad >> quad & 1) poison = 0xffff;
-        uint32_t w[kCols];
-#pragma unroll
-        for (int j = 0; j < kCols; ++j) {
-          const float base = ref[j] == -INFINITY ? 0.f : ref[j];
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            float x = exp2_fast(v[2 * j + r] - base);
-            if (poison >> ((lane >> 2) + 8 * r) & 1) x = __int_as_float(0x7fc00000);
-            if (edge && mine + 8 * r >= limit[j]) x = 0.f;
-            v[2 * j + r] = x;
-          }
-          sum[j] += v[2 * j] + v[2 * j + 1];
-        }
-#pragma unroll
-        for (int j = 0; j < kCols; j += 2) {
-          w[j] = Pair<T>::r(v[2 * j], v[2 * j + 2]);          // position lane / 4
-          w[j + 1] = Pair<T>::r(v[2 * j + 1], v[2 * j + 3]);  // ... + 8
-        }
-        // transposed 8 x 8 blocks: a row of queries has its 64 weights in 128 bytes, 16-byte pieces swizzled by the row
-#pragma unroll
-        for (int j = 0; j < N / 16; ++j) {
-          const int row = 16 * j + 8 * (lane >> 4) + (lane & 7), piece16 = 2 * quad + ((lane >> 3) & 1);
-          asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(
-                           smem_u32(S.p) + row * 128 + ((piece16 ^ (row & 7)) << 4)),
-                       "r"(w[4 * j]), "r"(w[4 * j + 1]), "r"(w[4 * j + 2]), "r"(w[4 * j + 3])
-                       : "memory");
-        }
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&S.p_full);
-      }
-      // sums of the weights over the positions, through the place of the maxima of the tile before the last
-#pragma unroll
-      for (int j = 0; j < kCols; ++j)
-#pragma unroll
-        for (int x = 4; x < 32; x <<= 1) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], x);
-      if (lane < 4) {
-#pragma unroll
-        for (int j = 0; j < kCols; j += 2)
-          *reinterpret_cast<float2*>(&S.wmax[k & 1][quad][4 * j + 2 * lane]) = make_float2(sum[j], sum[j + 1]);
-      }
-      asm volatile("bar.sync 1, 128;" ::: "memory");  // the last correction's factors are read
-      if (lane < 4 && quad == 0) {
-#pragma unroll
-        for (int j = 0; j < kCols; ++j) S.fac[4 * (j & ~1) + 2 * lane + (j & 1)] = ref[j];
-      }
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      const bool whole = p.whole && A.groups == 0;
-      const int slot = p.rt + c;  // pieces of the launch in order: either grows
-      if (slot >= P.slots) atomicExch(err, GEMQ_LATENT_BAD_LENGTH);
-      // thread 32 quad + lane: dimension 128 m + that of all rows of queries; first its row's sums
-      const int me = 32 * quad + lane;
-      const float(&lsum)[4][N] = S.wmax[k & 1];
-      if (me < p.rows && (whole || slot < P.slots)) {
-        const float l = lsum[0][me] + lsum[1][me] + lsum[2][me] + lsum[3][me], m = S.fac[me];
-        if (whole) A.lse[p.row0 + me] = limit_of(A, p.x, prefix, p.row0 + me) > 0 ? (m + log2f(l)) * kLn2 : -INFINITY;
-        else P.part_ml[static_cast<long long>(slot) * N + me] = make_float2(m, l);
-      }
-      wait_for(&S.o_full, piece & 1, &S.abort, err);
-      tc_fence_after_sync();
-      for (int m = 0; m < blocks / 2; ++m)
-#pragma unroll 1
-        for (int j = 0; j < N; j += 16) {
-          uint32_t o[16];
-          tmem_load16(tmem + lanes + kTmemO + m * N + j, o);
-          tmem_loaded(o);
-          if (whole) {
-            T* out = static_cast<T*>(A.out) + static_cast<long long>(p.row0 + j) * A.rank + 128 * m + (me & ~1);
-#pragma unroll
-            for (int x = 0; x < 16; x += 2) {  // an even lane takes row x of a pair of dimensions, its neighbour row x + 1
-              const float give = __uint_as_float(lane & 1 ? o[x] : o[x + 1]), keep = __uint_as_float(lane & 1 ? o[x + 1] : o[x]);
-              const float got = __shfl_xor_sync(0xffffffffu, give, 1);
-              const int r = x + (lane & 1), col = j + r;
-              if (col < p.rows) {
-                const float l = lsum[0][col] + lsum[1][col] + lsum[2][col] + lsum[3][col];
-                const float f = l == 0.f && limit_of(A, p.x, prefix, p.row0 + col) <= 0 ? 0.f : 1.f / l;
-                *reinterpret_cast<uint32_t*>(out + r * static_cast<long long>(A.rank)) =
-                    lane & 1 ? Pair<T>::r(got * f, keep * f) : Pair<T>::r(keep * f, got * f);
-              }
-            }
-          } else if (slot < P.slots) {
-            float* out = P.part_o + (static_cast<long long>(slot) * N + j) * A.rank + 128 * m + me;
-#pragma unroll
-            for (int x = 0; x < 16; ++x)
-              if (j + x < p.rows) out[x * static_cast<long long>(A.rank)] = __uint_as_float(o[x]);
-          }
-        }
-      tc_fence_before_sync();
-      asm volatile("bar.sync 1, 128;" ::: "memory");  // sums and references are read
-      if (lane == 0) mbar_arrive(&S.o_free);
+      const uint32_t acc = tmem + kTmemO + piece % kOs * (4 * N);
+      if (N == 16 || p.rows <= 16) softmax_piece<T, N, 16>(S, P, p, k, piece, tmem, acc);
+      else if (N == 32 || p.rows <= 32) softmax_piece<T, N, N < 32 ? 16 : 32>(S, P, p, k, piece, tmem, acc);
+      else if (p.rows <= 48) softmax_piece<T, N, N < 64 ? 16 : 48>(S, P, p, k, piece, tmem, acc);
+      else softmax_piece<T, N, N < 64 ? 16 : 64>(S, P, p, k, piece, tmem, acc);
     }
   }
   tc_fence_before_sync();
@@ -663,90 +765,91 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
 }
 
 // ---- pieces of a row joined ---------------------------------------------------------------------------
-// 128 numbers of a row at a time: four warps take its pieces in turn and add in a fixed order.
+// A CTA a row: rank / 4 threads have four numbers each of every fourth piece (more at small ranks), the sums of the threads that share
+// numbers are added in a fixed order.
+constexpr int kJoinThreads = 512;
+
 template <typename T>
-__global__ void __launch_bounds__(128) latent_join_kernel(const __grid_constant__ Args P, int N) {
-  __shared__ float4 part[4][32];
-  __shared__ float part_l[4];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+__global__ void __launch_bounds__(kJoinThreads) latent_join_kernel(const __grid_constant__ Args P, int N, int sms) {
+  __shared__ float4 part[kJoinThreads];
+  __shared__ float part_l[kJoinThreads / 32];
   const gemq_latent_decode_t& A = P.a;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, per = A.steps * A.heads, cuts = A.rank / 128;
-  const int total = P.ctl[0], ctas = P.ctl[1];
-  const long long jobs = static_cast<long long>(A.batch) * per * cuts;
-  for (long long job = blockIdx.x; job < jobs; job += gridDim.x) {
-    const int row = static_cast<int>(job / cuts), cut = static_cast<int>(job % cuts);
+  const int lane = threadIdx.x & 31, per = A.steps * A.heads;
+  const int wide = A.rank / 4, sets = kJoinThreads / wide, set = static_cast<int>(threadIdx.x) / wide, at4 = static_cast<int>(threadIdx.x) % wide;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  bool waited = false;
+  for (int row = blockIdx.x; row < A.batch * per; row += gridDim.x) {
     const int b = row / per, hidden = A.steps - 1 - row % per / A.heads;
-    // runs of slots: of the group's prefix, of the sequence's own tiles
-    int slot[2] = {0, 0}, count[2] = {0, 0}, at[2] = {0, 0}, len = 0;
-    bool whole = false;
-    if (total > 0) {
-      if (A.groups > 0) {
-        int g = 0, hi = A.groups;  // the last group that begins at b or before (g < hi)
-        while (hi - g > 1) {
-          const int mid = (g + hi) >> 1;
-          if (start_of(A, mid) <= b) g = mid;
-          else hi = mid;
-        }
-        const Entry x = entry_of(A, g);
-        const int r = row - x.row0;
-        if (x.tiles > 0 && r >= 0 && r < x.rows) {
-          len += x.len;
-          const long long t = P.ctl[2 + 2 * g] + static_cast<long long>(r / N) * x.tiles;
-          const int c0 = cta_of(t, total, ctas), c1 = cta_of(t + x.tiles - 1, total, ctas);
-          slot[0] = P.ctl[3 + 2 * g] + r / N + c0;
-          count[0] = c1 - c0 + 1;
-          at[0] = r % N;
-        }
+    // the inputs are those of the kernel before, which had waited for them when it let this one begin
+    int g = -1, len = 0;
+    Entry x[2];
+    x[0] = {0, 0, 0, 0, 0};
+    if (A.groups > 0) {
+      int hi = A.groups;  // the last group that begins at b or before (g < hi)
+      for (g = 0; hi - g > 1;) {
+        const int mid = (g + hi) >> 1;
+        if (start_of(A, mid) <= b) g = mid;
+        else hi = mid;
       }
-      const int e = A.groups + b;
-      const Entry x = entry_of(A, e);
-      len += x.len;
-      if (x.tiles > 0) {
-        const int r = row - x.row0;
-        const long long t = P.ctl[2 + 2 * e] + static_cast<long long>(r / N) * x.tiles;
-        const int c0 = cta_of(t, total, ctas), c1 = cta_of(t + x.tiles - 1, total, ctas);
-        slot[1] = P.ctl[3 + 2 * e] + r / N + c0;
-        count[1] = c1 - c0 + 1;
-        at[1] = r % N;
-        whole = A.groups == 0 && c0 == c1;
+      x[0] = entry_of(A, g);
+      if (row < x[0].row0 || row >= x[0].row0 + x[0].rows) x[0].tiles = 0;
+      else len = x[0].len;
+    }
+    x[1] = entry_of(A, A.groups + b);
+    len += x[1].len;
+    if (!waited) {
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      waited = true;
+    }
+    const int total = P.ctl[0], ctas = ctas_of(total, sms);
+    int slot[2] = {0, 0}, count[2] = {0, 0}, at[2] = {0, 0};  // runs of slots: of the group's prefix, of the sequence's own tiles
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int e = k ? A.groups + b : g;
+      if (x[k].tiles > 0) {
+        const int r = row - x[k].row0, base = P.ctl[2 + 2 * e] + r / N * x[k].cost;
+        const int c0 = cta_of(base, 0, total, ctas), c1 = cta_of(base, x[k].tiles - 1, total, ctas);
+        slot[k] = P.ctl[3 + 2 * e] + r / N + c0;
+        count[k] = c1 - c0 + 1;
+        at[k] = r % N;
       }
     }
-    if (whole) continue;  // written already
+    if (A.groups == 0 && count[1] == 1) continue;  // written already
     const int pieces = count[0] + count[1];
+    const long long rows = static_cast<long long>(P.slots) * N;
     auto place = [&](int i) -> long long {  // row of the scratch
       return i < count[0] ? static_cast<long long>(slot[0] + i) * N + at[0] : static_cast<long long>(slot[1] + i - count[0]) * N + at[1];
     };
-    const long long rows = static_cast<long long>(P.slots) * N;
     float top = -INFINITY;
     for (int i = lane; i < pieces; i += 32)
       if (place(i) < rows) top = fmaxf(top, P.part_ml[place(i)].x);
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
     const float base = top == -INFINITY ? 0.f : top;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     float l = 0.f;
-#pragma unroll 4
-    for (int i = warp; i < pieces; i += 4) {
-      const long long q = place(i);
-      if (q >= rows) continue;
-      const float2 ml = P.part_ml[q];
-      const float4 v = reinterpret_cast<const float4*>(P.part_o + q * A.rank + cut * 128)[lane];
-      const float f = exp2_fast(ml.x - base);
-      l = fmaf(ml.y, f, l);
-      o.x = fmaf(v.x, f, o.x);
-      o.y = fmaf(v.y, f, o.y);
-      o.z = fmaf(v.z, f, o.z);
-      o.w = fmaf(v.w, f, o.w);
+    if (set < sets) {
+#pragma unroll 8
+      for (int i = set; i < pieces; i += sets) {
+        const long long q = place(i);
+        if (q >= rows) continue;
+        const float2 ml = P.part_ml[q];
+        const float4 v = reinterpret_cast<const float4*>(P.part_o + q * A.rank)[at4];
+        const float f = exp2_fast(ml.x - base);
+        l = fmaf(ml.y, f, l);
+        o.x = fmaf(v.x, f, o.x);
+        o.y = fmaf(v.y, f, o.y);
+        o.z = fmaf(v.z, f, o.z);
+        o.w = fmaf(v.w, f, o.w);
+      }
+      part[threadIdx.x] = o;
+      if (at4 == 0) part_l[set] = l;
     }
-    part[warp][lane] = o;
-    if (lane == 0) part_l[warp] = l;
     __syncthreads();
-    if (warp == 0) {
-      l = part_l[0] + part_l[1] + part_l[2] + part_l[3];
-#pragma unroll
-      for (int w = 1; w < 4; ++w) {
-        const float4 v = part[w][lane];
+    if (set == 0) {
+      for (int s = 1; s < sets; ++s) {
+        const float4 v = part[s * wide + at4];
+        l += part_l[s];
         o.x += v.x;
         o.y += v.y;
         o.z += v.z;
@@ -754,9 +857,9 @@ __global__ void __launch_bounds__(128) latent_join_kernel(const __grid_constant_
       }
       const bool empty = len - hidden <= 0;
       const float f = 1.f / l;
-      reinterpret_cast<uint2*>(static_cast<T*>(A.out) + static_cast<long long>(row) * A.rank + cut * 128)[lane] =
+      reinterpret_cast<uint2*>(static_cast<T*>(A.out) + static_cast<long long>(row) * A.rank)[at4] =
           empty ? make_uint2(0, 0) : make_uint2(Pair<T>::r(o.x * f, o.y * f), Pair<T>::r(o.z * f, o.w * f));
-      if (lane == 0 && cut == 0) A.lse[row] = empty ? -INFINITY : (top + log2f(l)) * kLn2;
+      if (at4 == 0) A.lse[row] = empty ? -INFINITY : (top + log2f(l)) * kLn2;
     }
     __syncthreads();
   }
@@ -771,8 +874,8 @@ int check(const gemq_latent_decode_t* A) {
   if (rows > (1 << 30) || A->groups > (1 << 24)) return GEMQ_ERR_BAD_SHAPE;
   // the list of work is counted in 32 bits
   const long long own = static_cast<long long>(A->table_pitch) * A->page_size, pre = static_cast<long long>(A->prefix_pitch) * A->page_size;
-  const long long tiles = (rows / 16 + A->batch) * (own / kTile + 1) + (A->groups ? (rows / 16 + A->groups) * (pre / kTile + 1) : 0);
-  if (own > 0x7fffff00 || pre > 0x7fffff00 || tiles > 0x7fffffff) return GEMQ_ERR_BAD_SHAPE;
+  const long long tiles = (rows / 16 + A->batch) * (own / kTile + 2) + (A->groups ? (rows / 16 + A->groups) * (pre / kTile + 2) : 0);
+  if (own > 0x7fffff00 || pre > 0x7fffff00 || tiles > 0x7fffffff / 8) return GEMQ_ERR_BAD_SHAPE;
   if (!aligned16(A->q_latent) || !aligned16(A->q_rope) || !aligned16(A->cache) || !aligned16(A->out) || (A->page_stride & 7))
     return GEMQ_ERR_ALIGN;
   for (int i = 0; i < 3; ++i)
@@ -822,11 +925,11 @@ int launch(const Args& P, int ctas, cudaStream_t st) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   if (cudaLaunchKernelEx(&cfg, latent_decode_kernel<T, N>, P) != cudaSuccess) return GEMQ_ERR_LAUNCH;
-  const long long jobs = static_cast<long long>(P.a.batch) * P.a.steps * P.a.heads * (P.a.rank / 128), most = 8ll * ctas;
-  cfg.gridDim = dim3(static_cast<unsigned>(jobs < most ? jobs : most));
-  cfg.blockDim = dim3(128);
+  const long long rows = static_cast<long long>(P.a.batch) * P.a.steps * P.a.heads, most = 4ll * ctas;
+  cfg.gridDim = dim3(static_cast<unsigned>(rows < most ? rows : most));
+  cfg.blockDim = dim3(kJoinThreads);
   cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, latent_join_kernel<T>, P, N) == cudaSuccess ? GEMQ_OK : GEMQ_ERR_LAUNCH;
+  return cudaLaunchKernelEx(&cfg, latent_join_kernel<T>, P, N, ctas) == cudaSuccess ? GEMQ_OK : GEMQ_ERR_LAUNCH;
 }
 
 template <typename T>
