@@ -80,7 +80,6 @@ struct Args {
   float2* part_ml;   // [slots][N]: reference of the weights (in powers of two) and their sum
   int slots;
   float scale;       // times log2 e
-  int box_blocks;    // latent blocks of a TMA box: 2, or 1 where pages are shorter than a tile
 };
 
 // ---- the list of work -----------------------------------------------------------------------------
@@ -124,13 +123,21 @@ struct Piece {
   __device__ __forceinline__ bool whole() const { return n == x.tiles; }
 };
 
+// The same in all lanes, and known to be so: what the TMA and MMA instructions take stays in uniform registers.
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+
 template <int N>
 struct Walk {
   const gemq_latent_decode_t& A;
   Start s;
   Entry x;
-  __device__ __forceinline__ Walk(const gemq_latent_decode_t& a, const Start& at) : A(a), s(at) {
-    if (s.from < s.to) x = entry_of(A, s.e);
+  __device__ __forceinline__ Walk(const gemq_latent_decode_t& a, const Start& at)
+      : A(a), s{uniform(at.e), uniform(at.rt), uniform(at.base), uniform(at.from), uniform(at.to), uniform(at.rto)} {
+    if (s.from < s.to) enter();
+  }
+  __device__ __forceinline__ void enter() {
+    const Entry y = entry_of(A, s.e);
+    x = {uniform(y.len), uniform(y.tiles), uniform(y.row0), uniform(y.rows), uniform(y.cost)};
   }
   __device__ __forceinline__ bool next(Piece& p) {
     while (s.base < s.to && s.from < s.to) {
@@ -138,7 +145,7 @@ struct Walk {
         s.rto += cdiv(x.rows, N);
         s.rt = 0;
         if (++s.e >= A.groups + A.batch) { s.to = s.from; return false; }
-        x = entry_of(A, s.e);
+        enter();
         continue;
       }
       const int t0 = min(max((s.from - s.base - kPieceCost + 3) >> 2, 0), x.tiles);
@@ -413,29 +420,24 @@ __device__ __forceinline__ void softmax_piece(Smem<N>& S, const Args& P, const P
 }
 
 // ---- the warps at a piece's two ends ------------------------------------------------------------------
-// Its queries: eight lanes a row's 128 bytes of a block.
+// Its queries: eight lanes a row's 128 bytes of a block, all copies in flight.
 template <typename T, int N>
 __device__ __forceinline__ void load_queries(Smem<N>& S, const gemq_latent_decode_t& A, const Piece& p, uint32_t piece) {
-  const int tid = static_cast<int>(threadIdx.x) - 32 * kEdgeWarp, per = A.steps * A.heads, blocks = A.rank / 64, chunks = A.rank / 8 + 8;
+  const int tid = static_cast<int>(threadIdx.x) - 32 * kEdgeWarp, per = A.steps * A.heads, blocks = A.rank / 64;
   wait_for(&S.q_free, (piece & 1) ^ 1, &S.abort, A.err);
   for (int r = tid >> 3; r < p.width(); r += 16) {
     const int row = p.row0 + r, b = row / per, i = row % per / A.heads, h = row % A.heads;
-    const bool on = r < p.rows;
     const uint4* ql = reinterpret_cast<const uint4*>(static_cast<const T*>(A.q_latent) + b * A.q_latent_stride[0] + i * A.q_latent_stride[1] +
                                                      h * A.q_latent_stride[2]);
     const uint4* qr = reinterpret_cast<const uint4*>(static_cast<const T*>(A.q_rope) + b * A.q_rope_stride[0] + i * A.q_rope_stride[1] +
                                                      h * A.q_rope_stride[2]);
-    uint4 v[9];
-#pragma unroll
-    for (int d = 0; d < 9; ++d) {
-      const int at = d * 8 + (tid & 7);
-      v[d] = make_uint4(0, 0, 0, 0);
-      if (on && at < chunks) v[d] = at < chunks - 8 ? ql[at] : qr[at - (chunks - 8)];
+    const uint32_t dst = smem_u32(S.q[0]) + r * 128 + (((tid & 7) ^ (r & 7)) << 4), bytes = r < p.rows ? 16 : 0;  // 0: zeros
+    for (int d = 0; d <= blocks; ++d) {
+      const uint4* src = d < blocks ? ql + d * 8 + (tid & 7) : qr + (tid & 7);
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + d * (N * 128)), "l"(bytes ? static_cast<const void*>(src) : A.q_latent), "r"(bytes) : "memory");
     }
-#pragma unroll
-    for (int d = 0; d < 9; ++d)
-      if (d <= blocks) *reinterpret_cast<uint4*>(S.q[d] + r * 128 + (((tid & 7) ^ (r & 7)) << 4)) = v[d];
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
   fence_async_smem();
   __syncwarp();
   if ((tid & 31) == 0) mbar_arrive(&S.q_full);
@@ -520,6 +522,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) tmem_alloc(&S.tmem_base, kTmemCols);
+  if (warp == 0 && lane < 2) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<unsigned long long>(lane ? &P.rope_map : &P.latent_map)) : "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   // Every CTA adds up the list: a thread has a run of entries.
@@ -593,7 +596,9 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     uint32_t k = 0, phase = 1;
     const bool small = A.page_size < kTile;
     const int per_tile = small ? kTile / A.page_size : 1, quarters = small ? A.page_size / 16 : 4, tiles_a_page = small ? 1 : A.page_size / kTile;
-    const int box_rows = min(A.page_size, kTile), boxes = 2 / P.box_blocks;
+    const int box_rows = min(A.page_size, kTile);
+    const uint32_t ring0 = smem_u32(S.ring[0]), rope0 = smem_u32(S.rope[0]), full0 = smem_u32(&S.full[0]), rope_full0 = smem_u32(&S.rope_full[0]);
+    int rope_at = 0;
     while (walk.next(p)) {
       const bool prefix = p.e < A.groups;
       const int* table = prefix ? A.prefix_table + static_cast<long long>(p.e) * A.prefix_pitch
@@ -618,32 +623,61 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
           if (bad) atomicExch(err, GEMQ_LATENT_BAD_PAGE);
         }
         const uint32_t bytes = here * box_rows * 128;
-        int id[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) id[j] = __shfl_sync(0xffffffffu, out ? 0 : ids, (pg - base + j) & 31);
-        for (int d = 0; d < blocks; d += 2) {
-          wait_for(&S.empty[place >> 1], phase, &S.abort, err);
-          unsigned char* dst = S.ring[place];
-          unsigned long long* bar = &S.full[place >> 1];
+        if (!small) {
+          const int id = __shfl_sync(0xffffffffu, out ? 0 : ids, pg - base);
+          for (int d = 0; d < blocks; d += 2) {
+            wait_for(&S.empty[place >> 1], phase, &S.abort, err);
+            if (elect_lane()) {
+              mbar_expect_at(full0 + place * 4, 2 * kBlock);
+              tma_load_4d_at(ring0 + place * kBlock, &P.latent_map, row, d, id, full0 + place * 4);
+            }
+            __syncwarp();
+            place += 2;
+            if (place == kLatent) { place = 0; phase ^= 1; }
+          }
+          if (static_cast<int>(k) >= kRopes + freed) {
+            wait_for(&S.done[freed % kSlots], (freed / kSlots) & 1, &S.abort, err);
+            ++freed;
+          }
           if (elect_lane()) {
-            mbar_arrive_expect_tx(bar, 2 * bytes);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (j < here)
-                for (int n = 0; n < boxes; ++n) tma_load_4d(dst + n * kBlock + j * A.page_size * 128, &P.latent_map, 0, row, d + n, id[j], bar);
+            mbar_expect_at(rope_full0 + rope_at * 8, kBlock);
+            tma_load_4d_at(rope0 + rope_at * kBlock, &P.rope_map, row, blocks, id, rope_full0 + rope_at * 8);
           }
           __syncwarp();
-          place += 2;
-          if (place == kLatent) { place = 0; phase ^= 1; }
-        }
-        for (; static_cast<int>(k) >= kRopes + freed; ++freed) wait_for(&S.done[freed % kSlots], (freed / kSlots) & 1, &S.abort, err);
-        if (elect_lane()) {
-          mbar_arrive_expect_tx(&S.rope_full[k % kRopes], bytes);
+        } else {
+          int id[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (j < here) tma_load_4d(S.rope[k % kRopes] + j * A.page_size * 128, &P.rope_map, 0, row, blocks, id[j], &S.rope_full[k % kRopes]);
+          for (int j = 0; j < 4; ++j) id[j] = __shfl_sync(0xffffffffu, out ? 0 : ids, (pg - base + j) & 31);
+          const uint32_t page_bytes = A.page_size * 128;
+          for (int d = 0; d < blocks; d += 2) {
+            wait_for(&S.empty[place >> 1], phase, &S.abort, err);
+            const uint32_t dst = ring0 + place * kBlock, bar = full0 + place * 4;
+            if (elect_lane()) {
+              mbar_expect_at(bar, 2 * bytes);
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (j < here) {
+                  tma_load_4d_at(dst + j * page_bytes, &P.latent_map, 0, d, id[j], bar);
+                  tma_load_4d_at(dst + kBlock + j * page_bytes, &P.latent_map, 0, d + 1, id[j], bar);
+                }
+            }
+            __syncwarp();
+            place += 2;
+            if (place == kLatent) { place = 0; phase ^= 1; }
+          }
+          if (static_cast<int>(k) >= kRopes + freed) {
+            wait_for(&S.done[freed % kSlots], (freed / kSlots) & 1, &S.abort, err);
+            ++freed;
+          }
+          if (elect_lane()) {
+            mbar_expect_at(rope_full0 + rope_at * 8, bytes);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (j < here) tma_load_4d_at(rope0 + rope_at * kBlock + j * page_bytes, &P.rope_map, 0, blocks, id[j], rope_full0 + rope_at * 8);
+          }
+          __syncwarp();
         }
-        __syncwarp();
+        if (++rope_at == kRopes) rope_at = 0;
         if (small) {
           pg += per_tile;
         } else {
@@ -965,9 +999,8 @@ extern "C" int gemq_latent_decode(const gemq_latent_decode_t* A, void* scratch, 
   P.slots = s.slots;
   P.scale = A->scale * kLog2e;
   const int rows = A->page_size < kTile ? A->page_size : kTile;
-  P.box_blocks = A->page_size < kTile ? 1 : 2;
   const int blocks = A->rank / 64 + 1;
-  if (!tensor_map_pages(&P.latent_map, A->cache, blocks, A->page_size, A->page_stride, A->n_pages, rows, P.box_blocks) ||
+  if (!tensor_map_pages(&P.latent_map, A->cache, blocks, A->page_size, A->page_stride, A->n_pages, rows, A->page_size < kTile ? 1 : 2) ||
       !tensor_map_pages(&P.rope_map, A->cache, blocks, A->page_size, A->page_stride, A->n_pages, rows, 1))
     return GEMQ_ERR_LAUNCH;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

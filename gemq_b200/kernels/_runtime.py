@@ -77,15 +77,21 @@ def error_word(dev: torch.device) -> torch.Tensor:
 _err_ptrs: dict = {}
 
 
+def host_error_word(x):
+    """Address of the error word of x's device for the native calls, None on the CPU."""
+    i = x.get_device()
+    p = _err_ptrs.get(i)
+    if p is None and i >= 0:
+        p = _err_ptrs[i] = error_word(x.device).data_ptr()
+    return p
+
+
 def host_linear(x, w_q, scales, zeros, nbits, group_size, bias, mode: int):
     """The native call (csrc/host.cpp) or None.  ``mode``: 0 dense layer, 1 rows operator, 2 one-row operator,
     3 GEMM operator."""
-    i = x.get_device()
-    p = _err_ptrs.get(i)
+    p = host_error_word(x)
     if p is None:
-        if i < 0:
-            return None
-        p = _err_ptrs[i] = error_word(x.device).data_ptr()
+        return None
     return _capi.host.linear(x, w_q, scales, zeros, nbits, group_size, bias, p, mode)
 
 

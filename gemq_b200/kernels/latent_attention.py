@@ -20,7 +20,7 @@ from torch import Tensor
 
 from .. import _capi
 from ._ops import library_op
-from ._runtime import error_word, require, require_cuda, stream_ptr
+from ._runtime import error_word, host_error_word, require, require_cuda, stream_ptr
 
 ROPE, NOPE, VALUE = 64, 128, 128
 _HALF = (torch.float16, torch.bfloat16)
@@ -39,6 +39,14 @@ class _on:
     def __exit__(self, *a):
         if self.guard is not None:
             self.guard.__exit__(*a)
+
+
+def _native(name: str):
+    """The call in native code (csrc/host.cpp); None where it does not take the arguments, which the checks here then name."""
+    def fast(x, *rest):
+        p = host_error_word(x) if isinstance(x, Tensor) else None
+        return None if p is None else getattr(_capi.host, name)(p, x, *rest)
+    return fast
 
 
 def latent_error(device=None) -> int:
@@ -81,7 +89,7 @@ def _fake_append(kv, q_rope, norm_weight, eps, inv_freq, positions, slots, cache
     return q_rope.new_empty(q_rope.shape), kv.new_empty(kv.shape)
 
 
-@library_op("latent_append", _fake_append, mutates=("cache",))
+@library_op("latent_append", _fake_append, _native("latent_append"), mutates=("cache",))
 def latent_append(kv: Tensor, q_rope: Tensor, norm_weight: Tensor, eps: float, inv_freq: Tensor, positions: Tensor, slots: Tensor,
                   cache: Tensor, rope_scale: float = 1.0) -> Tuple[Tensor, Tensor]:
     """``kv [T, rank + 64]`` (what the compressing projection gives) -> cached rows, ``q_rope [T, H, 64]`` -> rotated queries.
@@ -158,7 +166,7 @@ def _fake_decode(q_latent, q_rope, cache, *rest):
     return q_latent.new_empty(q_latent.shape), q_latent.new_empty(q_latent.shape[:3], dtype=torch.float32)
 
 
-@library_op("latent_decode", _fake_decode)
+@library_op("latent_decode", _fake_decode, _native("latent_decode"))
 def latent_decode(q_latent: Tensor, q_rope: Tensor, cache: Tensor, table: Tensor, lens: Tensor, scale: float) -> Tuple[Tensor, Tensor]:
     """Attention of the last ``S`` tokens of every sequence over its cached rows, in the latent space.
 
@@ -171,7 +179,14 @@ def latent_decode(q_latent: Tensor, q_rope: Tensor, cache: Tensor, table: Tensor
     return _decode(q_latent, q_rope, cache, table, lens, scale)
 
 
-@library_op("latent_decode_shared", _fake_decode)
+def _native_shared(*a):
+    if len(a) != 9:
+        return None
+    q_latent, q_rope, cache, table, lens, prefix_table, prefix_lens, starts, scale = a
+    return _native("latent_decode")(q_latent, q_rope, cache, table, lens, scale, prefix_table, prefix_lens, starts)
+
+
+@library_op("latent_decode_shared", _fake_decode, _native_shared)
 def latent_decode_shared(q_latent: Tensor, q_rope: Tensor, cache: Tensor, table: Tensor, lens: Tensor, prefix_table: Tensor,
                          prefix_lens: Tensor, starts: Tensor, scale: float) -> Tuple[Tensor, Tensor]:
     """``latent_decode`` for a batch in which sequences ``starts[g] .. starts[g + 1] - 1`` begin with the same ``prefix_lens[g]``
@@ -186,7 +201,7 @@ def _fake_prefill(q_nope, q_rope, kv, k_rope, cu_q, cu_k, scale, causal=True):
     return q_nope.new_empty(q_nope.shape), q_nope.new_empty(q_nope.shape[:2], dtype=torch.float32)
 
 
-@library_op("latent_prefill", _fake_prefill)
+@library_op("latent_prefill", _fake_prefill, _native("latent_prefill"))
 def latent_prefill(q_nope: Tensor, q_rope: Tensor, kv: Tensor, k_rope: Tensor, cu_q: Tensor, cu_k: Tensor, scale: float,
                    causal: bool = True) -> Tuple[Tensor, Tensor]:
     """Attention of prompts over expanded keys and values, sequences one behind the other.
@@ -234,6 +249,8 @@ def copy_pages(cache: Tensor, src: Tensor, dst: Tensor) -> None:
     four dimensions and more, ``[layers, pages, ..]``; the pages themselves contiguous, of any type, a multiple of 16 bytes.
     The destinations must be distinct, and no page may be both a source and a destination, but for ``src[i] == dst[i]``, which
     is left alone.  Ids outside the cache are reported and skipped."""
+    if _native("copy_pages")(cache, src, dst):
+        return
     dev = require_cuda(cache, src, dst)
     require(cache.dim() >= 2, "cache must be [pages, ..] or [layers, pages, ..]")
     layers = cache.shape[0] if cache.dim() >= 4 else 1
