@@ -1,7 +1,7 @@
 // What the latent attention kernels share: 16-bit types, and where the rows of a sequence lie.
 #pragma once
 
-#include "common.cuh"
+#include "ptx.cuh"
 
 namespace gemq {
 namespace latent {
@@ -49,6 +49,43 @@ __device__ __forceinline__ bool offsets_ok(const int* v, int n, int most, bool t
   }
   return ok && (!to_the_end || last == most);
 }
+
+// A wait that runs out (about a second) is reported and ends all waits of the CTA.
+__device__ __forceinline__ void wait_for(unsigned long long* bar, uint32_t parity, int* abort, int* err) {
+  if (mbar_test_wait(bar, parity)) return;
+  for (int i = 0; i < (1 << 16); ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(20000)
+        : "memory");
+    if (ok || *reinterpret_cast<volatile int*>(abort)) return;
+  }
+  *reinterpret_cast<volatile int*>(abort) = 1;
+  atomicExch(err, GEMQ_LATENT_WAIT);
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Two numbers, eight of them: an infinity or a NaN among them.
+template <typename T>
+__device__ __forceinline__ bool has_nonfinite(uint32_t w) {
+  constexpr uint32_t kExp = Pair<T>::kBf16 ? 0x7f80u : 0x7c00u;
+  return (w & kExp) == kExp || ((w >> 16) & kExp) == kExp;
+}
+template <typename T>
+__device__ __forceinline__ bool has_nonfinite(uint4 v) {
+  return has_nonfinite<T>(v.x) || has_nonfinite<T>(v.y) || has_nonfinite<T>(v.z) || has_nonfinite<T>(v.w);
+}
+// The same in all lanes, and known to be so: what the TMA and MMA instructions take stays in uniform registers.
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 }  // namespace latent
 }  // namespace gemq

@@ -23,7 +23,6 @@
 // sequence.  Rows behind what is seen are zeroed in shared memory before they are multiplied by weights of 0: what lies there may be NaN.
 // Every wait is bounded.
 #include "latent.cuh"
-#include "ptx.cuh"
 
 namespace gemq {
 
@@ -123,9 +122,6 @@ struct Piece {
   __device__ __forceinline__ bool whole() const { return n == x.tiles; }
 };
 
-// The same in all lanes, and known to be so: what the TMA and MMA instructions take stays in uniform registers.
-__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
-
 template <int N>
 struct Walk {
   const gemq_latent_decode_t& A;
@@ -172,31 +168,6 @@ __device__ __forceinline__ int limit_of(const gemq_latent_decode_t& A, const Ent
   return x.len - max(hidden - clamp_length(A.lens[b], A.table_pitch, A.page_size, A.err), 0);
 }
 
-// ---- waits ------------------------------------------------------------------------------------------
-// A wait that runs out (about a second) is reported and ends all waits of the CTA.
-__device__ __forceinline__ void wait_for(unsigned long long* bar, uint32_t parity, int* abort, int* err) {
-  if (mbar_test_wait(bar, parity)) return;
-  for (int i = 0; i < (1 << 16); ++i) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity), "r"(20000)
-        : "memory");
-    if (ok || *reinterpret_cast<volatile int*>(abort)) return;
-  }
-  *reinterpret_cast<volatile int*>(abort) = 1;
-  atomicExch(err, GEMQ_LATENT_WAIT);
-}
-
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // Whether any of the 128 softmax threads says so; a barrier of theirs.
 __device__ __forceinline__ bool any_of_softmax(bool mine) {
   uint32_t any;
@@ -209,18 +180,6 @@ __device__ __forceinline__ bool any_of_softmax(bool mine) {
       : "r"(static_cast<uint32_t>(mine))
       : "memory");
   return any != 0;
-}
-
-template <typename T>
-__device__ __forceinline__ bool has_nonfinite(uint4 v) {
-  constexpr uint32_t kExp = Pair<T>::kBf16 ? 0x7f80u : 0x7c00u;
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t w = reinterpret_cast<const uint32_t*>(&v)[i];
-    bad |= (w & kExp) == kExp || ((w >> 16) & kExp) == kExp;
-  }
-  return bad;
 }
 
 // ---- the softmax warps: one piece ---------------------------------------------------------------------

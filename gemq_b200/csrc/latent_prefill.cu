@@ -2,67 +2,408 @@
 //
 //   s[i, j] = scale * (q_nope[i] . k_nope[j] + q_rope[i] . k_rope[j]),   out[i] = sum_j softmax(s)[i, j] v[j],   j <= i + keys - queries
 //
-// A warp a query row of one head; running maximum and sum in 32 bits.
+// What bounds it: 640 operations for each visible (query, key) of a head, against 16 to 32 exponentials a clock of a multiprocessor for one
+// each: the tensor cores, with the exponentials close behind (a 128 x 128 tile: 1280 cycles of MMAs, 1024 of ex2).
+//
+// A CTA has 256 queries of one head as two tiles of 128, each with a warp group for its softmax (a thread has a row), over the same
+// tiles of 128 keys: while the exponentials of one tile are formed the MMAs of the other run.  Scores, and in their place the weights
+// (16 bits), and the sums stay in tensor memory: 2 x (128 + 128) columns, all of it.
+//   warp 0      TMA: queries once, then two places of keys (48 KB) and one of values (32 KB)
+//   warp 1      MMAs: O0 of tile j, S0 of tile j + 1, O1 of tile j, S1 of tile j + 1
+//   warps 4-7, 8-11   softmax of either tile, results
+// The reference of a row's weights moves only when its scores exceed it by 2^8; then its sums are corrected in tensor memory.
+//
+// What a query must not see is given a weight of 0.  If such a row of v holds an infinity or a NaN the product still is NaN: a block with a
+// result that is not finite is computed once more, and warps 2 and 3 set to zero, in the tiles that not all of its queries see whole, what
+// is hidden from all and what is not finite; a query that sees one of the latter gets a NaN for its weight.  Every wait is bounded.
 #include "latent.cuh"
 
 namespace gemq {
+
+// tma.cu
+bool tensor_map_heads(CUtensorMap* out, const void* base, int width, int heads, long long head_stride, long long rows, long long row_stride,
+                      int box_rows);
+
 namespace latent {
 namespace {
 
-constexpr int kWarps = 8;
 constexpr int kNope = 128, kValue = 128;
+constexpr int kRows = 128;                 // of a tile: queries, and keys
+constexpr int kBlock = kRows * 128;        // bytes of 128 rows x 64 numbers
+constexpr int kThreads = 384, kSoftWarp = 4;
+
+constexpr int kAllKeys = 0x40000000;
+struct Item { int row0, rows, k0, keys, first; };  // query rows, key rows; what the first query sees (none if not above 0), or kAllKeys
+
+struct Smem {
+  alignas(1024) unsigned char q[2][3][kBlock];
+  unsigned char k[2][3][kBlock];
+  unsigned char v[2][kBlock];
+  alignas(8) unsigned long long q_full[2], k_full[2], k_free[2], v_full, v_free, v_clean, s_full[2], p_full[2], o_full[2];
+  uint32_t poison[4];
+  Item item;
+  uint32_t tmem_base;
+  int abort;
+};
+static_assert(sizeof(Smem) <= 232448, "more shared memory than a CTA has");
+
+struct Args {
+  CUtensorMap q_nope, q_rope, kv, k_rope;
+  gemq_latent_prefill_t a;
+  float scale;  // times log2 e
+};
+
+// Whether any thread of the CTA says so; all its threads come here.
+__device__ __forceinline__ bool any_in_cta(bool mine) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, 0, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any)
+      : "r"(static_cast<uint32_t>(mine))
+      : "memory");
+  return any != 0;
+}
+
+__device__ __forceinline__ int within(int v, int most) { return min(max(v, 0), most); }
 
 template <typename T>
-__global__ void __launch_bounds__(32 * kWarps) latent_prefill_row_kernel(const gemq_latent_prefill_t P) {
-  const int lane = threadIdx.x & 31;
-  const long long at = blockIdx.x * static_cast<long long>(kWarps) + (threadIdx.x >> 5);
-  const int row = static_cast<int>(at / P.heads), h = static_cast<int>(at % P.heads);
-  if (row >= P.q_rows) return;
-  if (at == 0 && lane == 0 && !(offsets_ok(P.cu_q, P.batch, P.q_rows, false) && offsets_ok(P.cu_k, P.batch, P.k_rows, false)))
-    atomicExch(P.err, GEMQ_LATENT_BAD_LENGTH);
-  int b = -1;
-  for (int i = 0; i < P.batch; ++i)
-    if (row >= P.cu_q[i] && row < P.cu_q[i + 1]) { b = i; break; }
-  int limit = 0, k0 = 0;
-  if (b >= 0) {
-    const int q0 = P.cu_q[b], q1 = P.cu_q[b + 1];
-    int k1 = P.cu_k[b + 1];
-    k0 = P.cu_k[b];
-    if (k0 < 0 || k1 < k0 || k1 > P.k_rows) {
-      if (lane == 0) atomicExch(P.err, GEMQ_LATENT_BAD_LENGTH);
-      k0 = max(k0, 0);
-      k1 = max(min(k1, P.k_rows), k0);
+__global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __grid_constant__ Args P) {
+  constexpr float kOffset = Pair<T>::kBf16 ? 0.f : 7.f;  // fp16 weights are 2^7 times as large: those above 2^-21 keep all their bits
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  Smem& S = *reinterpret_cast<Smem*>(smem_raw);
+  const gemq_latent_prefill_t& A = P.a;
+  int* const err = A.err;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int head = blockIdx.x % A.heads, at = blockIdx.x / A.heads;  // at: blocks of 256 queries, the last of a sequence first
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&S.q_full[i], 1);
+      mbar_init(&S.k_full[i], 1);
+      mbar_init(&S.k_free[i], 1);
+      mbar_init(&S.s_full[i], 1);
+      mbar_init(&S.p_full[i], 4);
+      mbar_init(&S.o_full[i], 1);
     }
-    limit = P.causal ? row - q0 + 1 + (k1 - k0) - (q1 - q0) : k1 - k0;
+    mbar_init(&S.v_full, 1);
+    mbar_init(&S.v_free, 1);
+    mbar_init(&S.v_clean, 2);
+    S.abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  const T* qn = static_cast<const T*>(P.q_nope) + row * P.q_nope_stride[0] + h * P.q_nope_stride[1];
-  const T* qr = static_cast<const T*>(P.q_rope) + row * P.q_rope_stride[0] + h * P.q_rope_stride[1];
-  const uint2 qv = reinterpret_cast<const uint2*>(qn)[lane];
-  const float2 q0 = Pair<T>::f(qv.x), q1 = Pair<T>::f(qv.y), q2 = Pair<T>::f(reinterpret_cast<const uint32_t*>(qr)[lane]);
-  float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int j = 0; j < limit; ++j) {
-    const T* kv = static_cast<const T*>(P.kv) + (k0 + j) * P.kv_stride[0] + h * P.kv_stride[1];
-    const uint2 kn = reinterpret_cast<const uint2*>(kv)[lane], v = reinterpret_cast<const uint2*>(kv + kNope)[lane];
-    const float2 a = Pair<T>::f(kn.x), c = Pair<T>::f(kn.y);
-    const float2 d = Pair<T>::f(reinterpret_cast<const uint32_t*>(static_cast<const T*>(P.k_rope) + (k0 + j) * P.k_rope_stride)[lane]);
-    float s = q0.x * a.x + q0.y * a.y + q1.x * c.x + q1.y * c.y + q2.x * d.x + q2.y * d.y;
+  if (warp == 1) tmem_alloc(&S.tmem_base, 512);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (warp == 0) {
+    // The block's sequence: 32 sequences at a time.  Behind the last there is one more, of the query rows that no sequence has.
+    int seen = 0;
+    bool found = false;
+    for (int b0 = 0; b0 <= A.batch && !found; b0 += 32) {
+      const int b = b0 + lane;
+      int q0 = 0, n = 0, k0 = 0, keys = 0;
+      if (b <= A.batch) {
+        q0 = within(A.cu_q[b], A.q_rows);
+        n = (b < A.batch ? within(A.cu_q[b + 1], A.q_rows) : A.q_rows) - q0;
+        k0 = within(A.cu_k[b], A.k_rows);
+        keys = b < A.batch ? max(within(A.cu_k[b + 1], A.k_rows) - k0, 0) : 0;
+      }
+      const int mine = n > 0 ? cdiv(n, 2 * kRows) : 0;
+      int upto = mine;
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    s *= P.scale;
-    const float now = fmaxf(m, s), base = now == -INFINITY ? 0.f : now;
-    const float f = __expf(m - base), p = __expf(s - base);
-    m = now;
-    l = fmaf(l, f, p);
-    const float2 v0 = Pair<T>::f(v.x), v1 = Pair<T>::f(v.y);
-    o[0] = fmaf(o[0], f, p * v0.x);
-    o[1] = fmaf(o[1], f, p * v0.y);
-    o[2] = fmaf(o[2], f, p * v1.x);
-    o[3] = fmaf(o[3], f, p * v1.y);
+      for (int d = 1; d < 32; d <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += v;
+      }
+      const bool hit = at >= seen + upto - mine && at < seen + upto;
+      if (hit) {
+        const int r0 = (seen + upto - 1 - at) * 2 * kRows;
+        S.item = {q0 + r0, min(n - r0, 2 * kRows), k0, keys, A.causal ? r0 + 1 + keys - n : kAllKeys};
+      }
+      found = __any_sync(0xffffffffu, hit);
+      seen += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    if (!found && lane == 0) S.item = {0, 0, 0, 0, 0};
   }
-  const long long out = static_cast<long long>(row) * P.heads + h;
-  const float r = limit > 0 ? 1.f / l : 0.f;
-  reinterpret_cast<uint2*>(static_cast<T*>(P.out) + out * kValue)[lane] = make_uint2(Pair<T>::r(o[0] * r, o[1] * r), Pair<T>::r(o[2] * r, o[3] * r));
-  if (lane == 0) P.lse[out] = limit > 0 ? m + logf(l) : -INFINITY;
+  if (blockIdx.x == 0 && threadIdx.x == 32 * 11 && !(offsets_ok(A.cu_q, A.batch, A.q_rows, false) && offsets_ok(A.cu_k, A.batch, A.k_rows, false)))
+    atomicExch(err, GEMQ_LATENT_BAD_LENGTH);
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  // Only now: a CTA of the next kernel must not take this SM's tensor memory first.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const uint32_t tmem = S.tmem_base;
+  const int row0 = uniform(S.item.row0), rows = uniform(S.item.rows), k0 = uniform(S.item.k0), keys = uniform(S.item.keys), first = uniform(S.item.first);
+  // query i of the block sees keys 0 .. limit(i) - 1
+  auto limit_of = [&](int i) { return first == kAllKeys ? keys : min(first + i, keys); };
+  int tiles[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int n = min(rows - t * kRows, kRows);
+    tiles[t] = n > 0 ? cdiv(max(limit_of(t * kRows + n - 1), 0), kRows) : 0;
+  }
+  const int most = max(tiles[0], tiles[1]);
+
+  // A second pass goes on with the barriers: how often each was completed in the first.
+  const int k_uses[2] = {(most + 1) >> 1, most >> 1};
+  const int least_of_all = max(limit_of(0), 0), most_of_all = max(limit_of(max(rows, 1) - 1), 0);
+  if (warp < kSoftWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == 0) {
+      const uint32_t q = smem_u32(S.q[0][0]), k = smem_u32(S.k[0][0]), v = smem_u32(S.v[0]);
+      auto load_q = [&](int t) {
+        const uint32_t bar = smem_u32(&S.q_full[t]), dst = q + t * 3 * kBlock;
+        const int r = row0 + t * kRows;
+        if (elect_lane()) {
+          mbar_expect_at(bar, 3 * kBlock);
+          tma_load_3d_at(dst, &P.q_nope, 0, head, r, bar);
+          tma_load_3d_at(dst + kBlock, &P.q_nope, 64, head, r, bar);
+          tma_load_3d_at(dst + 2 * kBlock, &P.q_rope, 0, head, r, bar);
+        }
+        __syncwarp();
+      };
+      for (int pass = 0;; ++pass) {
+        auto load_k = [&](int j) {
+          const int s = j & 1;
+          wait_for(&S.k_free[s], ((pass * k_uses[s] + (j >> 1)) & 1) ^ 1, &S.abort, err);
+          const uint32_t bar = smem_u32(&S.k_full[s]), dst = k + s * 3 * kBlock;
+          const int r = k0 + j * kRows;
+          if (elect_lane()) {
+            mbar_expect_at(bar, 3 * kBlock);
+            tma_load_3d_at(dst, &P.kv, 0, head, r, bar);
+            tma_load_3d_at(dst + kBlock, &P.kv, 64, head, r, bar);
+            tma_load_3d_at(dst + 2 * kBlock, &P.k_rope, 0, 0, r, bar);
+          }
+          __syncwarp();
+        };
+        if (most > 0) {
+          if (pass == 0 && tiles[0] > 0) load_q(0);
+          load_k(0);
+          if (pass == 0 && tiles[1] > 0) load_q(1);
+          for (int j = 0; j < most; ++j) {
+            if (j + 1 < most) load_k(j + 1);
+            wait_for(&S.v_free, ((pass * most + j) & 1) ^ 1, &S.abort, err);
+            const uint32_t bar = smem_u32(&S.v_full);
+            if (elect_lane()) {
+              mbar_expect_at(bar, 2 * kBlock);
+              tma_load_3d_at(v, &P.kv, kNope, head, k0 + j * kRows, bar);
+              tma_load_3d_at(v + kBlock, &P.kv, kNope + 64, head, k0 + j * kRows, bar);
+            }
+            __syncwarp();
+          }
+        }
+        if (!any_in_cta(false) || pass == 1) break;
+      }
+      // The copies in flight end before the CTA does: the MMAs waited for all of them, unless a wait ran out.
+      if (*reinterpret_cast<volatile int*>(&S.abort))
+        for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+    } else if (warp == 1) {
+      const uint32_t idesc_s = umma_idesc_f16(Pair<T>::kBf16, kRows, kRows), idesc_o = umma_idesc_f16(Pair<T>::kBf16, kRows, kValue) | kUmmaTransposeB;
+      const uint64_t q = umma_desc_k_sw128(smem_u32(S.q[0][0])), k = umma_desc_k_sw128(smem_u32(S.k[0][0])),
+                     v = umma_desc_mn_sw128(smem_u32(S.v[0]), kBlock);
+      for (int pass = 0;; ++pass) {
+        auto scores = [&](int t, int j) {
+          const int s = j & 1;
+          wait_for(&S.k_full[s], (pass * k_uses[s] + (j >> 1)) & 1, &S.abort, err);
+          tc_fence_after_sync();
+          const uint64_t a = q + t * (3 * kBlock >> 4), b = k + s * (3 * kBlock >> 4);
+          if (elect_lane()) {
+#pragma unroll
+            for (int i = 0; i < 12; ++i)
+              umma_ss_f16(tmem + t * kRows, a + (i >> 2) * (kBlock >> 4) + (i & 3) * 2, b + (i >> 2) * (kBlock >> 4) + (i & 3) * 2, idesc_s, i != 0);
+            umma_commit(&S.s_full[t]);
+            if (t == 1 || j >= tiles[1]) umma_commit(&S.k_free[s]);
+          }
+          __syncwarp();
+        };
+        auto sums = [&](int t, int j) {
+          wait_for(&S.p_full[t], (pass * tiles[t] + j) & 1, &S.abort, err);
+          wait_for(pass ? &S.v_clean : &S.v_full, j & 1, &S.abort, err);
+          tc_fence_after_sync();
+          const uint32_t o = tmem + 2 * kRows + t * kValue, p = tmem + t * kRows;
+          if (elect_lane()) {
+#pragma unroll
+            for (int i = 0; i < kRows / 16; ++i) umma_ts_f16_one(o, p + i * 8, v + i * (2048 >> 4), idesc_o, j != 0 || i != 0);
+            if (t == 1 || j >= tiles[1]) umma_commit(&S.v_free);
+            if (j == tiles[t] - 1) umma_commit(&S.o_full[t]);
+          }
+          __syncwarp();
+        };
+        for (int t = 0; t < 2; ++t)
+          if (tiles[t] > 0) {
+            wait_for(&S.q_full[t], 0, &S.abort, err);
+            scores(t, 0);
+          }
+        for (int j = 0; j < most; ++j)
+          for (int t = 0; t < 2; ++t) {
+            if (j < tiles[t]) sums(t, j);
+            if (j + 1 < tiles[t]) scores(t, j + 1);
+          }
+        if (!any_in_cta(false) || pass == 1) break;
+      }
+    } else if (any_in_cta(false)) {
+      // second pass: a warp has 64 rows of a tile of v
+      const int r0 = (warp - 2) * 64;
+      for (int j = 0; j < most; ++j) {
+        wait_for(&S.v_full, (most + j) & 1, &S.abort, err);
+        uint32_t poison[2] = {0, 0};
+        for (int r = max(least_of_all - j * kRows - r0, 0); r < 64; ++r) {
+          uint2* at = reinterpret_cast<uint2*>(S.v[lane >> 4] + (r0 + r) * 128) + (lane & 15);
+          bool wipe = j * kRows + r0 + r >= most_of_all;
+          if (!wipe) {
+            const uint2 x = *at;
+            wipe = __any_sync(0xffffffffu, has_nonfinite<T>(x.x) || has_nonfinite<T>(x.y));
+            if (wipe) poison[r >> 5] |= 1u << (r & 31);
+          }
+          if (wipe) *at = make_uint2(0, 0);
+        }
+        if (lane == 0) {
+          S.poison[2 * (warp - 2)] = poison[0];
+          S.poison[2 * (warp - 2) + 1] = poison[1];
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&S.v_clean);
+      }
+      any_in_cta(false);
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int t = (warp - kSoftWarp) >> 2, quad = warp & 3, i = t * kRows + 32 * quad + lane;
+    const uint32_t lanes = static_cast<uint32_t>(32 * quad) << 16, s = tmem + lanes + t * kRows, o = tmem + lanes + 2 * kRows + t * kValue;
+    const int limit = limit_of(i), least = limit_of(t * kRows + 32 * quad);
+    for (int pass = 0;; ++pass) {
+      float ref = 0.f, sum = 0.f;
+      bool none = true;
+      for (int j = 0; j < tiles[t]; ++j) {
+        wait_for(&S.s_full[t], (pass * tiles[t] + j) & 1, &S.abort, err);
+        tc_fence_after_sync();
+        uint32_t raw[kRows];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_load32(s + 32 * c, raw + 32 * c);
+        tmem_loaded(raw);
+        float* v = reinterpret_cast<float*>(raw);
+#pragma unroll
+        for (int c = 0; c < kRows; ++c) v[c] = fmaf(v[c], P.scale, -ref);
+        if (pass) {
+          wait_for(&S.v_clean, j & 1, &S.abort, err);
+#pragma unroll
+          for (int c = 0; c < kRows; ++c)
+            if (S.poison[c >> 5] >> (c & 31) & 1) v[c] = __int_as_float(0x7fc00000);
+        }
+        if ((j + 1) * kRows > least) {
+          const int here = limit - j * kRows;
+#pragma unroll
+          for (int c = 0; c < kRows; ++c)
+            if (c >= here) v[c] = -INFINITY;
+        }
+        float top = fmaxf(v[0], v[1]);
+#pragma unroll
+        for (int c = 2; c < kRows; c += 2) top = fmaxf(top, fmaxf(v[c], v[c + 1]));
+        if (__any_sync(0xffffffffu, none ? top > -INFINITY : top > kOffset + 8.f)) {
+          const float up = none ? top - kOffset : fmaxf(top - kOffset, 0.f), by = up == -INFINITY ? 0.f : up;
+          const float f = none ? 1.f : exp2_fast(-by);
+          none = none && up == -INFINITY;
+          ref += by;
+          sum *= f;
+#pragma unroll
+          for (int c = 0; c < kRows; ++c) v[c] -= by;
+          if (j > 0) {
+#pragma unroll
+            for (int c = 0; c < kValue; c += 16) {
+              uint32_t x[16];
+              tmem_load16(o + c, x);
+              tmem_loaded(x);
+#pragma unroll
+              for (int y = 0; y < 16; ++y) x[y] = __float_as_uint(__uint_as_float(x[y]) * f);
+              tmem_store16(o + c, x);
+            }
+          }
+        }
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < kRows; c += 32) {
+          uint32_t w[16];
+#pragma unroll
+          for (int y = 0; y < 16; ++y) {
+            const float a = exp2_fast(v[c + 2 * y]), b = exp2_fast(v[c + 2 * y + 1]);
+            part[y & 3] += a + b;
+            w[y] = Pair<T>::r(a, b);
+          }
+          tmem_store16(s + c / 2, w);
+        }
+        sum += (part[0] + part[1]) + (part[2] + part[3]);
+        tmem_stored();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&S.p_full[t]);
+      }
+      bool bad = false;
+      if (t * kRows + 32 * quad < rows) {  // the warp has rows
+        const bool on = i < rows;
+        const long long out = static_cast<long long>(row0 + i) * A.heads + head;
+        T* const to = static_cast<T*>(A.out) + out * kValue;
+        if (tiles[t] > 0) {
+          wait_for(&S.o_full[t], pass, &S.abort, err);
+          tc_fence_after_sync();
+          const float f = limit > 0 ? 1.f / sum : 0.f;
+          float check = 0.f;
+#pragma unroll 1
+          for (int c = 0; c < kValue; c += 16) {
+            uint32_t x[16], w[8];
+            tmem_load16(o + c, x);
+            tmem_loaded(x);
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+              const float a = __uint_as_float(x[2 * y]) * f, b = __uint_as_float(x[2 * y + 1]) * f;
+              check += (a - a) + (b - b);  // 0, or NaN
+              w[y] = Pair<T>::r(a, b);
+            }
+            if (on) {
+              reinterpret_cast<uint4*>(to + c)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+              reinterpret_cast<uint4*>(to + c)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+            }
+          }
+          bad = on && check != 0.f;
+        } else if (on) {
+          for (int c = 0; c < kValue; c += 8) *reinterpret_cast<uint4*>(to + c) = make_uint4(0, 0, 0, 0);
+        }
+        if (on) A.lse[out] = limit > 0 && tiles[t] > 0 ? (ref + log2f(sum)) * kLn2 : -INFINITY;
+      }
+      tc_fence_before_sync();
+      // where all rows see all of the tiles a second pass would find the same
+      if (!any_in_cta(bad && least_of_all < most * kRows) || pass == 1) break;
+      tc_fence_after_sync();
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <typename T>
+int launch(const Args& P, unsigned ctas, cudaStream_t st) {
+  static bool set[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return GEMQ_ERR_LAUNCH;
+  if (!set[dev]) {
+    if (cudaFuncSetAttribute(latent_prefill_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Smem)) != cudaSuccess) return GEMQ_ERR_LAUNCH;
+    set[dev] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = sizeof(Smem);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, latent_prefill_kernel<T>, P) == cudaSuccess ? GEMQ_OK : GEMQ_ERR_LAUNCH;
 }
 
 }  // namespace
@@ -78,18 +419,29 @@ extern "C" int gemq_latent_prefill(const gemq_latent_prefill_t* A, gemq_stream_t
   if (!A->q_nope || !A->q_rope || !A->cu_q || !A->cu_k || !A->out || !A->lse || !A->err || A->batch < 0 || A->q_rows < 0 || A->k_rows < 0 ||
       A->heads <= 0 || (A->k_rows && (!A->kv || !A->k_rope)))
     return GEMQ_ERR_BAD_ARG;
-  if (static_cast<long long>(A->q_rows) * A->heads > (1ll << 31)) return GEMQ_ERR_BAD_SHAPE;
+  const long long blocks = (A->q_rows / (2ll * kRows) + A->batch + 1) * A->heads;
+  if (blocks > 0x7fffffff || A->q_rows > 0x3fffffff || A->k_rows > 0x3fffffff) return GEMQ_ERR_BAD_SHAPE;
   for (const void* p : {A->q_nope, A->q_rope, A->kv, A->k_rope, static_cast<const void*>(A->out)})
     if (p && !aligned16(p)) return GEMQ_ERR_ALIGN;
   if ((A->q_nope_stride[0] | A->q_nope_stride[1] | A->q_rope_stride[0] | A->q_rope_stride[1] | A->kv_stride[0] | A->kv_stride[1] |
        A->k_rope_stride) & 7)
     return GEMQ_ERR_ALIGN;
-  const long long rows = static_cast<long long>(A->q_rows) * A->heads;
-  const unsigned grid = static_cast<unsigned>((rows + kWarps - 1) / kWarps);
+  // a tiled copy has no stride of 0
+  if (A->q_rows > 1 && (A->q_nope_stride[0] <= 0 || A->q_rope_stride[0] <= 0)) return GEMQ_ERR_BAD_SHAPE;
+  if (A->k_rows > 1 && (A->kv_stride[0] <= 0 || A->k_rope_stride <= 0)) return GEMQ_ERR_BAD_SHAPE;
+  if (A->heads > 1 && (A->q_nope_stride[1] <= 0 || A->q_rope_stride[1] <= 0 || (A->k_rows && A->kv_stride[1] <= 0))) return GEMQ_ERR_BAD_SHAPE;
+  Args P;
+  P.a = *A;
+  P.scale = A->scale * kLog2e;
+  // without keys no tile is loaded: any valid map does
+  const void* kv = A->k_rows ? A->kv : A->q_nope;
+  const void* kr = A->k_rows ? A->k_rope : A->q_rope;
+  const long long kn = A->k_rows ? A->k_rows : 1;
+  if (!tensor_map_heads(&P.q_nope, A->q_nope, kNope, A->heads, A->q_nope_stride[1], A->q_rows, A->q_nope_stride[0], kRows) ||
+      !tensor_map_heads(&P.q_rope, A->q_rope, kRope, A->heads, A->q_rope_stride[1], A->q_rows, A->q_rope_stride[0], kRows) ||
+      !tensor_map_heads(&P.kv, kv, A->k_rows ? kNope + kValue : 64, A->k_rows ? A->heads : 1, A->kv_stride[1], kn, A->kv_stride[0], kRows) ||
+      !tensor_map_heads(&P.k_rope, kr, kRope, 1, 0, kn, A->k_rope_stride, kRows))
+    return GEMQ_ERR_LAUNCH;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (A->is_bf16)
-    latent_prefill_row_kernel<__nv_bfloat16><<<grid, 32 * kWarps, 0, st>>>(*A);
-  else
-    latent_prefill_row_kernel<__half><<<grid, 32 * kWarps, 0, st>>>(*A);
-  return launch_status();
+  return A->is_bf16 ? launch<__nv_bfloat16>(P, static_cast<unsigned>(blocks), st) : launch<__half>(P, static_cast<unsigned>(blocks), st);
 }

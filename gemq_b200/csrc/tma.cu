@@ -142,4 +142,19 @@ bool tensor_map_pages(CUtensorMap* out, const void* base, int blocks, int page_s
              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// 16-bit rows [rows, heads, width] as (width, head, row): a box brings 64 numbers of `box_rows` rows of one head, 128-byte swizzle.  Strides
+// in elements; those of a dimension of 1 do not count.  Made anew for every call.
+bool tensor_map_heads(CUtensorMap* out, const void* base, int width, int heads, long long head_stride, long long rows, long long row_stride,
+                      int box_rows) {
+  EncodeTiledFn enc = encode_tiled_fn();
+  if (!enc) return false;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[2] = {heads > 1 ? static_cast<cuuint64_t>(head_stride) * 2 : static_cast<cuuint64_t>(width) * 2,
+                                 rows > 1 ? static_cast<cuuint64_t>(row_stride) * 2 : static_cast<cuuint64_t>(width) * 2};
+  const cuuint32_t box[3] = {64, 1, static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t estr[3] = {1u, 1u, 1u};
+  return enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }  // namespace gemq

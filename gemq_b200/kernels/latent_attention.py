@@ -228,6 +228,9 @@ def latent_prefill(q_nope: Tensor, q_rope: Tensor, kv: Tensor, k_rope: Tensor, c
     lse = torch.empty((Tq, H), dtype=torch.float32, device=dev)
     if Tq == 0:
         return out, lse
+    # a tiled copy has no stride of 0: what is expanded is laid out
+    q_nope, q_rope, kv, k_rope = (t.contiguous() if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())) else t
+                                  for t in (q_nope, q_rope, kv, k_rope))
     A = _capi.LatentPrefill()
     A.q_nope, A.q_nope_stride[:] = q_nope.data_ptr(), _strides("q_nope", q_nope)
     A.q_rope, A.q_rope_stride[:] = q_rope.data_ptr(), _strides("q_rope", q_rope)
