@@ -231,7 +231,7 @@ PyObject* latent_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   gemq_latent_decode_t A = {};
   const int64_t rank = cache_rank(c, *ql, &A.page_stride), B = ql->size(0), S = ql->size(1), H = ql->size(2);
   if (!rank || ql->size(3) != rank || B <= 0 || S <= 0 || H <= 0 || qr->size(0) != B || qr->size(1) != S || qr->size(2) != H || qr->size(3) != 64 ||
-      qr->scalar_type() != ql->scalar_type() || B * S * H > (1 << 30))
+      qr->scalar_type() != ql->scalar_type() || B * S * H > (1 << 28))
     return none();
   const auto dev = ql->device();
   if (!row_strides(*ql, A.q_latent_stride) || !row_strides(*qr, A.q_rope_stride)) return none();

@@ -51,8 +51,7 @@ __device__ __forceinline__ bool offsets_ok(const int* v, int n, int most, bool t
 }
 
 // A wait that runs out (about a second) is reported and ends all waits of the CTA.
-__device__ __forceinline__ void wait_for(unsigned long long* bar, uint32_t parity, int* abort, int* err) {
-  if (mbar_test_wait(bar, parity)) return;
+__device__ __forceinline__ void wait_here(uint32_t bar, uint32_t parity, int* abort, int* err) {
   for (int i = 0; i < (1 << 16); ++i) {
     uint32_t ok;
     asm volatile(
@@ -60,12 +59,37 @@ __device__ __forceinline__ void wait_for(unsigned long long* bar, uint32_t parit
         "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity), "r"(20000)
+        : "r"(bar), "r"(parity), "r"(20000)
         : "memory");
     if (ok || *reinterpret_cast<volatile int*>(abort)) return;
   }
   *reinterpret_cast<volatile int*>(abort) = 1;
   atomicExch(err, GEMQ_LATENT_WAIT);
+}
+// Out of line where it can be: the waits are many, and a launch that runs for 10 us spends half of its time on instructions that are not in
+// the cache yet.  (CALL: not in code that has asked for more registers, where a call cannot be allocated.)
+static __device__ __noinline__ void wait_on(uint32_t bar, uint32_t parity, int* abort, int* err) { wait_here(bar, parity, abort, err); }
+template <bool CALL = false>
+__device__ __forceinline__ void wait_for(unsigned long long* bar, uint32_t parity, int* abort, int* err) {
+  if (mbar_test_wait(bar, parity)) return;
+  if (CALL) wait_on(smem_u32(bar), parity, abort, err);
+  else wait_here(smem_u32(bar), parity, abort, err);
+}
+
+// Division of a 32-bit n >= 0 by a number of the launch: with l = ceil(log2 d) the multiplier floor(2^32 (2^l - d) / d) + 1 and 2^32 above it
+// give n / d after a shift by l, the sum halved on the way so that it fits.
+struct Div {
+  uint32_t mul;
+  int half, shift;
+  __device__ __forceinline__ int operator()(int n) const {
+    const uint32_t q = __umulhi(mul, static_cast<uint32_t>(n));
+    return static_cast<int>((((static_cast<uint32_t>(n) - q) >> half) + q) >> shift);
+  }
+};
+inline Div div_by(uint32_t d) {  // d > 0
+  int l = 0;
+  while ((1ull << l) < d) ++l;
+  return {static_cast<uint32_t>(((1ull << l) - d) * (1ull << 32) / d + 1), l > 0 ? 1 : 0, l > 0 ? l - 1 : 0};
 }
 
 __device__ __forceinline__ float exp2_fast(float x) {

@@ -37,8 +37,6 @@ constexpr int kTile = 64;            // positions of a tile
 constexpr int kBlock = kTile * 128;  // bytes of 64 positions x 64 numbers
 constexpr int kThreads = 384;
 constexpr int kSoftWarp = 4, kEdgeWarp = 8;  // four each: a warp reads the quarter of the tensor memory that its number names
-// What a piece costs beside its tiles, in quarters of a tile.
-constexpr int kPieceCost = 4;
 constexpr int kSlots = 8;            // tiles in flight that are told apart: one more than the rope blocks, 4, at most
 
 // Blocks of the ring: what 227 KB hold beside the queries.
@@ -79,15 +77,19 @@ struct Args {
   float2* part_ml;   // [slots][N]: reference of the weights (in powers of two) and their sum
   int slots;
   float scale;       // times log2 e
+  Div per, heads;    // query rows of a sequence; heads
 };
 
 // ---- the list of work -----------------------------------------------------------------------------
 __device__ __forceinline__ int start_of(const gemq_latent_decode_t& A, int g) {  // within the batch, whatever the device has
   return g <= 0 ? 0 : g >= A.groups ? A.batch : min(max(A.starts[g], 0), A.batch);
 }
-struct Entry { int len, tiles, row0, rows, cost; };  // positions, tiles of 64, first query row (of batch * steps * heads), query rows; of a row tile
+// Positions, tiles of 64, first query row (of batch * steps * heads), query rows; what a piece costs beside its tiles, in quarters of a tile, and
+// what a row tile costs.
+struct Entry { int len, tiles, row0, rows, piece, cost; };
 
-__device__ __forceinline__ Entry entry_of(const gemq_latent_decode_t& A, int e) {
+__device__ __forceinline__ Entry entry_here(const Args& P, int e) {
+  const gemq_latent_decode_t& A = P.a;
   const int per = A.steps * A.heads;
   Entry x;
   if (e < A.groups) {
@@ -102,16 +104,29 @@ __device__ __forceinline__ Entry entry_of(const gemq_latent_decode_t& A, int e) 
     x.len = clamp_length(A.lens[b], A.table_pitch, A.page_size, A.err);
   }
   x.tiles = cdiv(x.len, kTile);
-  x.cost = x.tiles ? 4 * x.tiles + kPieceCost : 0;
+  // Measured, two and more pieces of a CTA against one: 16 rows 3.4 us a piece and 2.2 a tile, 64 rows 6 us and 1.7.
+  x.piece = x.rows <= 32 ? 6 : 14;
+  x.cost = x.tiles ? 4 * x.tiles + x.piece : 0;
   return x;
 }
-// Tile t of a row tile that begins at `base` of the list is at base + kPieceCost + 4 t; CTA c of C has what lies in
-// floor(c T / C) .. floor((c + 1) T / C) - 1 of the list's T.
-// A share is a tile or more: no CTA between a row tile's first and last is without one.
-__device__ __forceinline__ int ctas_of(int total, int most) { return min(most, max(total / 4, 1)); }
-__device__ __forceinline__ int cta_of(int base, int t, int total, int ctas) {
-  return static_cast<int>((static_cast<long long>(base + kPieceCost + 4 * t + 1) * ctas - 1) / total);
-}
+// Out of line, as it is wanted in many places: see wait_on.
+__device__ __noinline__ Entry entry_of(const Args& P, int e) { return entry_here(P, e); }
+
+// Tile t of a row tile that begins at `base` of the list is at base + piece + 4 t.  The list is cut into shares of `share` or, the first
+// `longer` of them, one more.  A share is a tile or more: no CTA between a row tile's first and last is without one.
+struct Cut {
+  int ctas, share, longer;
+  __device__ __forceinline__ Cut(int total, int most) {
+    ctas = min(most, max(total / 4, 1));
+    share = total / ctas;
+    longer = total - share * ctas;
+  }
+  __device__ __forceinline__ int from(int c) const { return c * share + min(c, longer); }
+  __device__ __forceinline__ int cta_of(int at) const {
+    const int long_ones = longer * (share + 1);
+    return at < long_ones ? at / (share + 1) : longer + (at - long_ones) / share;
+  }
+};
 
 struct Piece {
   Entry x;
@@ -122,30 +137,30 @@ struct Piece {
   __device__ __forceinline__ bool whole() const { return n == x.tiles; }
 };
 
-template <int N>
+template <int N, bool CALL = true>
 struct Walk {
-  const gemq_latent_decode_t& A;
+  const Args& P;
   Start s;
   Entry x;
-  __device__ __forceinline__ Walk(const gemq_latent_decode_t& a, const Start& at)
-      : A(a), s{uniform(at.e), uniform(at.rt), uniform(at.base), uniform(at.from), uniform(at.to), uniform(at.rto)} {
+  __device__ __forceinline__ Walk(const Args& args, const Start& at)
+      : P(args), s{uniform(at.e), uniform(at.rt), uniform(at.base), uniform(at.from), uniform(at.to), uniform(at.rto)} {
     if (s.from < s.to) enter();
   }
   __device__ __forceinline__ void enter() {
-    const Entry y = entry_of(A, s.e);
-    x = {uniform(y.len), uniform(y.tiles), uniform(y.row0), uniform(y.rows), uniform(y.cost)};
+    const Entry y = CALL ? entry_of(P, s.e) : entry_here(P, s.e);
+    x = {uniform(y.len), uniform(y.tiles), uniform(y.row0), uniform(y.rows), uniform(y.piece), uniform(y.cost)};
   }
   __device__ __forceinline__ bool next(Piece& p) {
     while (s.base < s.to && s.from < s.to) {
       if (x.cost == 0 || s.rt * N >= x.rows) {
         s.rto += cdiv(x.rows, N);
         s.rt = 0;
-        if (++s.e >= A.groups + A.batch) { s.to = s.from; return false; }
+        if (++s.e >= P.a.groups + P.a.batch) { s.to = s.from; return false; }
         enter();
         continue;
       }
-      const int t0 = min(max((s.from - s.base - kPieceCost + 3) >> 2, 0), x.tiles);
-      const int t1 = min(max((s.to - s.base - kPieceCost + 3) >> 2, 0), x.tiles);
+      const int t0 = min(max((s.from - s.base - x.piece + 3) >> 2, 0), x.tiles);
+      const int t1 = min(max((s.to - s.base - x.piece + 3) >> 2, 0), x.tiles);
       p.x = x;
       p.e = s.e;
       p.t0 = t0;
@@ -161,11 +176,23 @@ struct Walk {
   }
 };
 
+// Sequence, step and head of a query row.
+struct Row {
+  int b, i, h;
+  __device__ __forceinline__ Row(const Args& P, int r) {
+    b = P.per(r);
+    const int rest = r - b * P.a.steps * P.a.heads;
+    i = P.heads(rest);
+    h = rest - i * P.a.heads;
+  }
+};
 // What query row r sees of entry e's positions.
-__device__ __forceinline__ int limit_of(const gemq_latent_decode_t& A, const Entry& x, bool prefix, int r) {
-  const int per = A.steps * A.heads, b = r / per, hidden = A.steps - 1 - (r % per) / A.heads;
+__device__ __forceinline__ int limit_of(const Args& P, const Entry& x, bool prefix, int r) {
+  const gemq_latent_decode_t& A = P.a;
+  const Row row(P, r);
+  const int hidden = A.steps - 1 - row.i;
   if (!prefix) return x.len - hidden;
-  return x.len - max(hidden - clamp_length(A.lens[b], A.table_pitch, A.page_size, A.err), 0);
+  return x.len - max(hidden - clamp_length(A.lens[row.b], A.table_pitch, A.page_size, A.err), 0);
 }
 
 // Whether any of the 128 softmax threads says so; a barrier of theirs.
@@ -200,7 +227,7 @@ __device__ __forceinline__ void softmax_piece(Smem<N>& S, const Args& P, const P
   for (int j = 0; j < kCols; ++j) ref[j] = sum[j] = 0.f;
   int least = p.x.len, most = 0;
   for (int r = lane; r < NP; r += 32) {
-    const int limit = r < p.rows ? limit_of(A, p.x, prefix, p.row0 + r) : 0;
+    const int limit = r < p.rows ? limit_of(P, p.x, prefix, p.row0 + r) : 0;
     if (quad == 0) S.limit[r] = limit;
     if (r < p.rows) {
       least = min(least, limit);
@@ -381,15 +408,16 @@ __device__ __forceinline__ void softmax_piece(Smem<N>& S, const Args& P, const P
 // ---- the warps at a piece's two ends ------------------------------------------------------------------
 // Its queries: eight lanes a row's 128 bytes of a block, all copies in flight.
 template <typename T, int N>
-__device__ __forceinline__ void load_queries(Smem<N>& S, const gemq_latent_decode_t& A, const Piece& p, uint32_t piece) {
-  const int tid = static_cast<int>(threadIdx.x) - 32 * kEdgeWarp, per = A.steps * A.heads, blocks = A.rank / 64;
-  wait_for(&S.q_free, (piece & 1) ^ 1, &S.abort, A.err);
+__device__ __forceinline__ void load_queries(Smem<N>& S, const Args& P, const Piece& p, uint32_t piece) {
+  const gemq_latent_decode_t& A = P.a;
+  const int tid = static_cast<int>(threadIdx.x) - 32 * kEdgeWarp, blocks = A.rank / 64;
+  wait_for<N != 64>(&S.q_free, (piece & 1) ^ 1, &S.abort, A.err);
   for (int r = tid >> 3; r < p.width(); r += 16) {
-    const int row = p.row0 + r, b = row / per, i = row % per / A.heads, h = row % A.heads;
-    const uint4* ql = reinterpret_cast<const uint4*>(static_cast<const T*>(A.q_latent) + b * A.q_latent_stride[0] + i * A.q_latent_stride[1] +
-                                                     h * A.q_latent_stride[2]);
-    const uint4* qr = reinterpret_cast<const uint4*>(static_cast<const T*>(A.q_rope) + b * A.q_rope_stride[0] + i * A.q_rope_stride[1] +
-                                                     h * A.q_rope_stride[2]);
+    const Row row(P, r < p.rows ? p.row0 + r : p.row0);
+    const uint4* ql = reinterpret_cast<const uint4*>(static_cast<const T*>(A.q_latent) + row.b * A.q_latent_stride[0] + row.i * A.q_latent_stride[1] +
+                                                     row.h * A.q_latent_stride[2]);
+    const uint4* qr = reinterpret_cast<const uint4*>(static_cast<const T*>(A.q_rope) + row.b * A.q_rope_stride[0] + row.i * A.q_rope_stride[1] +
+                                                     row.h * A.q_rope_stride[2]);
     const uint32_t dst = smem_u32(S.q[0]) + r * 128 + (((tid & 7) ^ (r & 7)) << 4), bytes = r < p.rows ? 16 : 0;  // 0: zeros
     for (int d = 0; d <= blocks; ++d) {
       const uint4* src = d < blocks ? ql + d * 8 + (tid & 7) : qr + (tid & 7);
@@ -412,41 +440,47 @@ __device__ __forceinline__ void finish_piece(Smem<N>& S, const Args& P, const Pi
   const bool prefix = p.e < A.groups, whole = p.whole() && A.groups == 0;
   const int slot = p.rt + static_cast<int>(blockIdx.x);  // pieces of the launch in order: either grows
   if (slot >= P.slots) atomicExch(A.err, GEMQ_LATENT_BAD_LENGTH);
-  wait_for(&S.r_full, piece & 1, &S.abort, A.err);
+  wait_for<N != 64>(&S.r_full, piece & 1, &S.abort, A.err);
   if (me < p.rows && (whole || slot < P.slots)) {
     const float2 r = S.result[me];
-    if (whole) A.lse[p.row0 + me] = limit_of(A, p.x, prefix, p.row0 + me) > 0 ? (r.x + log2f(r.y)) * kLn2 : -INFINITY;
-    else P.part_ml[static_cast<long long>(slot) * N + me] = r;
+    if (whole) {
+      const bool empty = limit_of(P, p.x, prefix, p.row0 + me) <= 0;
+      A.lse[p.row0 + me] = empty ? -INFINITY : (r.x + log2f(r.y)) * kLn2;
+      S.result[me].y = empty ? 0.f : __fdividef(1.f, r.y);
+    } else {
+      P.part_ml[static_cast<long long>(slot) * N + me] = r;
+    }
   }
-  wait_for(&S.o_full[piece % kOs], (piece / kOs) & 1, &S.abort, A.err);
+  if (whole) asm volatile("bar.sync 2, 128;" ::: "memory");  // the factors
+  wait_for<N != 64>(&S.o_full[piece % kOs], (piece / kOs) & 1, &S.abort, A.err);
   tc_fence_after_sync();
-  for (int m = 0; m < A.rank / 128; ++m)
 #pragma unroll 1
-    for (int j = 0; j < p.rows; j += 16) {
+  for (int j = 0; j < p.rows; j += 16) {
+    float f[8];  // of the rows that the thread stores: every second one
+#pragma unroll
+    for (int x = 0; x < 8; ++x) f[x] = whole ? S.result[j + 2 * x + (lane & 1)].y : 0.f;
+#pragma unroll 1
+    for (int m = 0; m < A.rank / 128; ++m) {
       uint32_t o[16];
       tmem_load16(acc + lanes + m * N + j, o);
       tmem_loaded(o);
       if (whole) {
-        T* out = static_cast<T*>(A.out) + static_cast<long long>(p.row0 + j) * A.rank + 128 * m + (me & ~1);
+        T* out = static_cast<T*>(A.out) + static_cast<long long>(p.row0 + j + (lane & 1)) * A.rank + 128 * m + (me & ~1);
 #pragma unroll
         for (int x = 0; x < 16; x += 2) {  // an even lane takes row x of a pair of dimensions, its neighbour row x + 1
           const float give = __uint_as_float(lane & 1 ? o[x] : o[x + 1]), keep = __uint_as_float(lane & 1 ? o[x + 1] : o[x]);
-          const float got = __shfl_xor_sync(0xffffffffu, give, 1);
-          const int r = x + (lane & 1), col = j + r;
-          if (col < p.rows) {
-            const float l = S.result[col].y;
-            const float f = l == 0.f && limit_of(A, p.x, prefix, p.row0 + col) <= 0 ? 0.f : 1.f / l;
-            *reinterpret_cast<uint32_t*>(out + r * static_cast<long long>(A.rank)) =
-                lane & 1 ? Pair<T>::r(got * f, keep * f) : Pair<T>::r(keep * f, got * f);
-          }
+          const float got = __shfl_xor_sync(0xffffffffu, give, 1), k = f[x >> 1];
+          const uint32_t w = lane & 1 ? Pair<T>::r(got * k, keep * k) : Pair<T>::r(keep * k, got * k);
+          if (j + x + (lane & 1) < p.rows) *reinterpret_cast<uint32_t*>(out + x * A.rank) = w;
         }
       } else if (slot < P.slots) {
         float* out = P.part_o + (static_cast<long long>(slot) * N + j) * A.rank + 128 * m + me;
 #pragma unroll
         for (int x = 0; x < 16; ++x)
-          if (j + x < p.rows) out[x * static_cast<long long>(A.rank)] = __uint_as_float(o[x]);
+          if (j + x < p.rows) out[x * A.rank] = __uint_as_float(o[x]);
       }
     }
+  }
   tc_fence_before_sync();
   __syncwarp();
   if (lane == 0) {
@@ -490,7 +524,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
   for (int k = 0; k < run; ++k) {
     const int e = static_cast<int>(threadIdx.x) * run + k;
     if (e >= entries) break;
-    const Entry x = entry_of(A, e);
+    const Entry x = entry_of(P, e);
     const int n = cdiv(x.rows, N);
     cost += n * x.cost;
     rts += n;
@@ -515,9 +549,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     if (w < warp) { before += S.sums[w][0]; rts_before += S.sums[w][1]; }
     total += S.sums[w][0];
   }
-  const int ctas = ctas_of(total, gridDim.x), c = blockIdx.x;
-  const int from = c < ctas ? static_cast<int>(static_cast<long long>(c) * total / ctas) : 0;
-  const int to = c < ctas ? static_cast<int>(static_cast<long long>(c + 1) * total / ctas) : 0;
+  const Cut cut(total, gridDim.x);
+  const int c = blockIdx.x, from = c < cut.ctas ? cut.from(c) : 0, to = c < cut.ctas ? cut.from(c + 1) : 0;
   if (c == 0 && threadIdx.x == 0) {
     P.ctl[0] = total;
     if (A.groups > 0 && !offsets_ok(A.starts, A.groups, A.batch, true)) atomicExch(A.err, GEMQ_LATENT_BAD_LENGTH);
@@ -527,7 +560,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     for (int k = 0; k < run; ++k) {
       const int e = static_cast<int>(threadIdx.x) * run + k;
       if (e >= entries) break;
-      const Entry x = entry_of(A, e);
+      const Entry x = entry_of(P, e);
       const int n = cdiv(x.rows, N), all = n * x.cost;
       if (c == 0) {
         P.ctl[2 + 2 * e] = at;
@@ -549,29 +582,29 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
   if (warp < kSoftWarp) {
   if (N == 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   if (warp == 0) {
-    Walk<N> walk(A, start);
+    Walk<N> walk(P, start);
     Piece p;
     int place = 0, freed = 0;  // next latent block of the ring; tiles known to be done
     uint32_t k = 0, phase = 1;
     const bool small = A.page_size < kTile;
     const int per_tile = small ? kTile / A.page_size : 1, quarters = small ? A.page_size / 16 : 4, tiles_a_page = small ? 1 : A.page_size / kTile;
-    const int box_rows = min(A.page_size, kTile);
+    const int box_rows = min(A.page_size, kTile), page_bits = A.page_size == 16 ? 4 : 5;  // of small pages
     const uint32_t ring0 = smem_u32(S.ring[0]), rope0 = smem_u32(S.rope[0]), full0 = smem_u32(&S.full[0]), rope_full0 = smem_u32(&S.rope_full[0]);
     int rope_at = 0;
     while (walk.next(p)) {
       const bool prefix = p.e < A.groups;
       const int* table = prefix ? A.prefix_table + static_cast<long long>(p.e) * A.prefix_pitch
                                 : A.table + static_cast<long long>(p.e - A.groups) * A.table_pitch;
-      const int pages = (p.x.len + A.page_size - 1) / A.page_size;
-      int pg = small ? p.t0 * per_tile : p.t0 / tiles_a_page, row = small ? 0 : (p.t0 % tiles_a_page) * kTile;
-      int base = pg, ids = base + lane < pages ? table[base + lane] : 0;  // lane i has the id of page base + i
+      const int pitch = prefix ? A.prefix_pitch : A.table_pitch;
+      int pg = small ? p.t0 * per_tile : tiles_a_page == 1 ? p.t0 : p.t0 / tiles_a_page, row = small ? 0 : (p.t0 - pg * tiles_a_page) * kTile;
+      int base = pg, ids = base + lane < pitch ? table[base + lane] : 0;  // lane i has the id of page base + i
       for (int i = 0; i < p.n; ++i, ++k) {
-        const int here = min(per_tile, pages - pg);  // pages of the tile
+        const int here = small ? (min(p.x.len - (p.t0 + i) * kTile, kTile) + A.page_size - 1) >> page_bits : 1;  // pages of the tile
         if (pg + here > base + 32) {
           base = pg;
-          ids = base + lane < pages ? table[base + lane] : 0;
+          ids = base + lane < pitch ? table[base + lane] : 0;
         }
-        const bool out = (ids < 0 || ids >= A.n_pages) && base + lane < pages;
+        const bool out = ids < 0 || ids >= A.n_pages;
         const uint32_t outs = __ballot_sync(0xffffffffu, out) >> (pg - base);
         int bad = 0;
         for (int j = 0; j < here; ++j)
@@ -585,7 +618,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
         if (!small) {
           const int id = __shfl_sync(0xffffffffu, out ? 0 : ids, pg - base);
           for (int d = 0; d < blocks; d += 2) {
-            wait_for(&S.empty[place >> 1], phase, &S.abort, err);
+            wait_for<N != 64>(&S.empty[place >> 1], phase, &S.abort, err);
             if (elect_lane()) {
               mbar_expect_at(full0 + place * 4, 2 * kBlock);
               tma_load_4d_at(ring0 + place * kBlock, &P.latent_map, row, d, id, full0 + place * 4);
@@ -595,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
             if (place == kLatent) { place = 0; phase ^= 1; }
           }
           if (static_cast<int>(k) >= kRopes + freed) {
-            wait_for(&S.done[freed % kSlots], (freed / kSlots) & 1, &S.abort, err);
+            wait_for<N != 64>(&S.done[freed % kSlots], (freed / kSlots) & 1, &S.abort, err);
             ++freed;
           }
           if (elect_lane()) {
@@ -609,7 +642,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
           for (int j = 0; j < 4; ++j) id[j] = __shfl_sync(0xffffffffu, out ? 0 : ids, (pg - base + j) & 31);
           const uint32_t page_bytes = A.page_size * 128;
           for (int d = 0; d < blocks; d += 2) {
-            wait_for(&S.empty[place >> 1], phase, &S.abort, err);
+            wait_for<N != 64>(&S.empty[place >> 1], phase, &S.abort, err);
             const uint32_t dst = ring0 + place * kBlock, bar = full0 + place * 4;
             if (elect_lane()) {
               mbar_expect_at(bar, 2 * bytes);
@@ -625,7 +658,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
             if (place == kLatent) { place = 0; phase ^= 1; }
           }
           if (static_cast<int>(k) >= kRopes + freed) {
-            wait_for(&S.done[freed % kSlots], (freed / kSlots) & 1, &S.abort, err);
+            wait_for<N != 64>(&S.done[freed % kSlots], (freed / kSlots) & 1, &S.abort, err);
             ++freed;
           }
           if (elect_lane()) {
@@ -650,7 +683,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
       for (int i = 0; i < 2000; ++i) __nanosleep(1000);
   } else if (warp == 1) {
     // The whole warp runs the loop and one elected lane issues: descriptors stay in uniform registers.
-    Walk<N> walk(A, start);
+    Walk<N> walk(P, start);
     Piece p;
     const uint64_t q0 = umma_desc_k_sw128(smem_u32(S.q[0])), ring0 = umma_desc_k_sw128(smem_u32(S.ring[0])),
                    rope0 = umma_desc_k_sw128(smem_u32(S.rope[0]));
@@ -658,12 +691,12 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     int place = 0;
     for (uint32_t piece = 0; walk.next(p); ++piece) {
       const uint32_t idesc = umma_idesc_f16(Pair<T>::kBf16, kTile, p.width());
-      wait_for(&S.q_full, piece & 1, &S.abort, err);
+      wait_for<N != 64>(&S.q_full, piece & 1, &S.abort, err);
       for (int i = 0; i < p.n; ++i, ++k) {
-        wait_for(&S.s_free[k & 1], ((k >> 1) & 1) ^ 1, &S.abort, err);
+        wait_for<N != 64>(&S.s_free[k & 1], ((k >> 1) & 1) ^ 1, &S.abort, err);
         const uint32_t s = tmem + (k & 1) * N;
         for (int d = 0; d < blocks; d += 2) {
-          wait_for(&S.full[place >> 1], phase, &S.abort, err);
+          wait_for<N != 64>(&S.full[place >> 1], phase, &S.abort, err);
           tc_fence_after_sync();
           const uint64_t a = ring0 + place * (kBlock >> 4), b = q0 + d * (N * 128 >> 4);
           if (elect_lane()) {
@@ -675,7 +708,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
           place += 2;
           if (place == kLatent) { place = 0; phase ^= 1; }
         }
-        wait_for(&S.rope_full[rope_at], rope_phase, &S.abort, err);
+        wait_for<N != 64>(&S.rope_full[rope_at], rope_phase, &S.abort, err);
         tc_fence_after_sync();
         const uint64_t a = rope0 + rope_at * (kBlock >> 4), b = q0 + blocks * (N * 128 >> 4);
         if (elect_lane()) {
@@ -689,7 +722,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
       }
     }
   } else if (warp == 2) {
-    Walk<N> walk(A, start);
+    Walk<N> walk(P, start);
     Piece p;
     const uint64_t p0 = umma_desc_k_sw128(smem_u32(S.p)), ring0 = umma_desc_mn_sw128(smem_u32(S.ring[0]), kBlock);
     uint32_t k = 0;
@@ -697,10 +730,10 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     for (uint32_t piece = 0; walk.next(p); ++piece) {
       const uint32_t idesc = umma_idesc_f16(Pair<T>::kBf16, 128, p.width()) | kUmmaTransposeA;
       const uint32_t acc = tmem + kTmemO + piece % kOs * (4 * N);
-      wait_for(&S.o_free[piece % kOs], ((piece / kOs) & 1) ^ 1, &S.abort, err);
+      wait_for<N != 64>(&S.o_free[piece % kOs], ((piece / kOs) & 1) ^ 1, &S.abort, err);
       for (int i = 0; i < p.n; ++i, ++k) {
         const int steps = cdiv(min(p.x.len - (p.t0 + i) * kTile, kTile), 16);  // of 16 positions
-        wait_for(&S.p_full, k & 1, &S.abort, err);
+        wait_for<N != 64>(&S.p_full, k & 1, &S.abort, err);
         tc_fence_after_sync();
         // a pair of blocks is free behind its MMAs: S of the tile is complete
         for (int m = 0; m < blocks / 2; ++m) {
@@ -728,17 +761,17 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     }
   }
   } else if (warp >= kEdgeWarp) {
-    Walk<N> ahead(A, start), walk(A, start);
+    Walk<N> ahead(P, start), walk(P, start);
     Piece q, p;
     uint32_t loads = 0;
-    if (ahead.next(q)) load_queries<T, N>(S, A, q, loads++);
+    if (ahead.next(q)) load_queries<T, N>(S, P, q, loads++);
     for (uint32_t piece = 0; walk.next(p); ++piece) {
-      if (ahead.next(q)) load_queries<T, N>(S, A, q, loads++);
+      if (ahead.next(q)) load_queries<T, N>(S, P, q, loads++);
       finish_piece<T, N>(S, P, p, piece, tmem + kTmemO + piece % kOs * (4 * N));
     }
   } else {
     if (N == 64) asm volatile("setmaxnreg.inc.sync.aligned.u32 240;");
-    Walk<N> walk(A, start);
+    Walk<N, N != 64> walk(P, start);
     Piece p;
     uint32_t k = 0;
     for (uint32_t piece = 0; walk.next(p); ++piece) {
@@ -758,25 +791,28 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
 }
 
 // ---- pieces of a row joined ---------------------------------------------------------------------------
-// A CTA a row: rank / 4 threads have four numbers each of every fourth piece (more at small ranks), the sums of the threads that share
-// numbers are added in a fixed order.
-constexpr int kJoinThreads = 512;
+// A warp has 128 numbers of a row, eight pieces in flight.  Many rows have few pieces each (W = 1): a CTA has a row, and its warps all pieces of
+// their numbers.  Few rows may have a piece from every CTA (W = 8): a CTA has 128 numbers, its warps take every eighth piece and keep a maximum
+// of their own; the eight are added in a fixed order.
+constexpr int kJoinAhead = 8;
 
-template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) latent_join_kernel(const __grid_constant__ Args P, int N, int sms) {
-  __shared__ float4 part[kJoinThreads];
-  __shared__ float part_l[kJoinThreads / 32];
+template <typename T, int W>
+__global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) latent_join_kernel(const __grid_constant__ Args P, int N, int sms) {
+  __shared__ float4 part[W][32];
+  __shared__ float2 part_ml[W];
   const gemq_latent_decode_t& A = P.a;
-  const int lane = threadIdx.x & 31, per = A.steps * A.heads;
-  const int wide = A.rank / 4, sets = kJoinThreads / wide, set = static_cast<int>(threadIdx.x) / wide, at4 = static_cast<int>(threadIdx.x) % wide;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cuts = A.rank / 128;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   bool waited = false;
-  for (int row = blockIdx.x; row < A.batch * per; row += gridDim.x) {
-    const int b = row / per, hidden = A.steps - 1 - row % per / A.heads;
+  const int per_row = W == 1 ? 1 : cuts;
+  for (int job = blockIdx.x; job < A.batch * A.steps * A.heads * per_row; job += gridDim.x) {
+    const int row = W == 1 ? job : cuts == 4 ? job >> 2 : job / cuts, at4 = (W == 1 ? warp : job - row * cuts) * 32 + lane;
+    const Row q(P, row);
+    const int b = q.b, hidden = A.steps - 1 - q.i;
     // the inputs are those of the kernel before, which had waited for them when it let this one begin
     int g = -1, len = 0;
     Entry x[2];
-    x[0] = {0, 0, 0, 0, 0};
+    x[0] = {0, 0, 0, 0, 0, 0};
     if (A.groups > 0) {
       int hi = A.groups;  // the last group that begins at b or before (g < hi)
       for (g = 0; hi - g > 1;) {
@@ -784,24 +820,24 @@ __global__ void __launch_bounds__(kJoinThreads) latent_join_kernel(const __grid_
         if (start_of(A, mid) <= b) g = mid;
         else hi = mid;
       }
-      x[0] = entry_of(A, g);
+      x[0] = entry_here(P, g);
       if (row < x[0].row0 || row >= x[0].row0 + x[0].rows) x[0].tiles = 0;
       else len = x[0].len;
     }
-    x[1] = entry_of(A, A.groups + b);
+    x[1] = entry_here(P, A.groups + b);
     len += x[1].len;
     if (!waited) {
       asm volatile("griddepcontrol.wait;" ::: "memory");
       waited = true;
     }
-    const int total = P.ctl[0], ctas = ctas_of(total, sms);
+    const Cut cut(P.ctl[0], sms);
     int slot[2] = {0, 0}, count[2] = {0, 0}, at[2] = {0, 0};  // runs of slots: of the group's prefix, of the sequence's own tiles
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const int e = k ? A.groups + b : g;
       if (x[k].tiles > 0) {
         const int r = row - x[k].row0, base = P.ctl[2 + 2 * e] + r / N * x[k].cost;
-        const int c0 = cta_of(base, 0, total, ctas), c1 = cta_of(base, x[k].tiles - 1, total, ctas);
+        const int c0 = cut.cta_of(base + x[k].piece), c1 = cut.cta_of(base + x[k].piece + 4 * (x[k].tiles - 1));
         slot[k] = P.ctl[3 + 2 * e] + r / N + c0;
         count[k] = c1 - c0 + 1;
         at[k] = r % N;
@@ -809,52 +845,70 @@ __global__ void __launch_bounds__(kJoinThreads) latent_join_kernel(const __grid_
     }
     if (A.groups == 0 && count[1] == 1) continue;  // written already
     const int pieces = count[0] + count[1];
-    const long long rows = static_cast<long long>(P.slots) * N;
-    auto place = [&](int i) -> long long {  // row of the scratch
-      return i < count[0] ? static_cast<long long>(slot[0] + i) * N + at[0] : static_cast<long long>(slot[1] + i - count[0]) * N + at[1];
-    };
-    float top = -INFINITY;
-    for (int i = lane; i < pieces; i += 32)
-      if (place(i) < rows) top = fmaxf(top, P.part_ml[place(i)].x);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    const float base = top == -INFINITY ? 0.f : top;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    float l = 0.f;
-    if (set < sets) {
-#pragma unroll 8
-      for (int i = set; i < pieces; i += sets) {
-        const long long q = place(i);
-        if (q >= rows) continue;
-        const float2 ml = P.part_ml[q];
-        const float4 v = reinterpret_cast<const float4*>(P.part_o + q * A.rank)[at4];
-        const float f = exp2_fast(ml.x - base);
-        l = fmaf(ml.y, f, l);
-        o.x = fmaf(v.x, f, o.x);
-        o.y = fmaf(v.y, f, o.y);
-        o.z = fmaf(v.z, f, o.z);
-        o.w = fmaf(v.w, f, o.w);
+    float l = 0.f, top = -INFINITY;
+    if (W == 1 && warp >= cuts) continue;
+    for (int i0 = W == 1 ? 0 : warp; i0 < pieces; i0 += W * kJoinAhead) {
+      float4 v[kJoinAhead];
+      float2 ml[kJoinAhead];
+#pragma unroll
+      for (int k = 0; k < kJoinAhead; ++k) {
+        const int i = i0 + W * k, s = i < count[0] ? slot[0] + i : slot[1] + i - count[0];
+        ml[k] = make_float2(-INFINITY, 0.f);
+        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i < pieces && s < P.slots) {
+          const long long from = static_cast<long long>(s) * N + (i < count[0] ? at[0] : at[1]);
+          ml[k] = P.part_ml[from];
+          v[k] = reinterpret_cast<const float4*>(P.part_o + from * A.rank)[at4];
+        }
       }
-      part[threadIdx.x] = o;
-      if (at4 == 0) part_l[set] = l;
+      float now = top;
+#pragma unroll
+      for (int k = 0; k < kJoinAhead; ++k) now = fmaxf(now, ml[k].x);
+      const float base = now == -INFINITY ? 0.f : now, f0 = exp2_fast(top - base);
+      top = now;
+      l *= f0;
+      o = make_float4(o.x * f0, o.y * f0, o.z * f0, o.w * f0);
+#pragma unroll
+      for (int k = 0; k < kJoinAhead; ++k) {
+        const float f = exp2_fast(ml[k].x - base);
+        l = fmaf(ml[k].y, f, l);
+        o.x = fmaf(v[k].x, f, o.x);
+        o.y = fmaf(v[k].y, f, o.y);
+        o.z = fmaf(v[k].z, f, o.z);
+        o.w = fmaf(v[k].w, f, o.w);
+      }
     }
-    __syncthreads();
-    if (set == 0) {
-      for (int s = 1; s < sets; ++s) {
-        const float4 v = part[s * wide + at4];
-        l += part_l[s];
-        o.x += v.x;
-        o.y += v.y;
-        o.z += v.z;
-        o.w += v.w;
+    if (W > 1) {
+      part[warp][lane] = o;
+      if (lane == 0) part_ml[warp] = make_float2(top, l);
+      __syncthreads();
+      if (warp == 0) {
+#pragma unroll
+        for (int w = 1; w < W; ++w) top = fmaxf(top, part_ml[w].x);
+        const float base = top == -INFINITY ? 0.f : top;
+        o = make_float4(0.f, 0.f, 0.f, 0.f);
+        l = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          const float4 v = part[w][lane];
+          const float f = exp2_fast(part_ml[w].x - base);
+          l = fmaf(part_ml[w].y, f, l);
+          o.x = fmaf(v.x, f, o.x);
+          o.y = fmaf(v.y, f, o.y);
+          o.z = fmaf(v.z, f, o.z);
+          o.w = fmaf(v.w, f, o.w);
+        }
       }
+    }
+    if (W == 1 || warp == 0) {
       const bool empty = len - hidden <= 0;
       const float f = 1.f / l;
       reinterpret_cast<uint2*>(static_cast<T*>(A.out) + static_cast<long long>(row) * A.rank)[at4] =
           empty ? make_uint2(0, 0) : make_uint2(Pair<T>::r(o.x * f, o.y * f), Pair<T>::r(o.z * f, o.w * f));
       if (at4 == 0) A.lse[row] = empty ? -INFINITY : (top + log2f(l)) * kLn2;
     }
-    __syncthreads();
+    if (W > 1) __syncthreads();
   }
 }
 
@@ -864,7 +918,7 @@ int check(const gemq_latent_decode_t* A) {
   if (A->groups && (!A->prefix_table || !A->prefix_lens || !A->starts || A->prefix_pitch < 0)) return GEMQ_ERR_BAD_ARG;
   if (!rank_ok(A->rank) || !page_ok(A->page_size)) return GEMQ_ERR_BAD_SHAPE;
   const long long rows = static_cast<long long>(A->batch) * A->steps * A->heads;
-  if (rows > (1 << 30) || A->groups > (1 << 24)) return GEMQ_ERR_BAD_SHAPE;
+  if (rows > (1 << 28) || A->groups > (1 << 24)) return GEMQ_ERR_BAD_SHAPE;
   // the list of work is counted in 32 bits
   const long long own = static_cast<long long>(A->table_pitch) * A->page_size, pre = static_cast<long long>(A->prefix_pitch) * A->page_size;
   const long long tiles = (rows / 16 + A->batch) * (own / kTile + 2) + (A->groups ? (rows / 16 + A->groups) * (pre / kTile + 2) : 0);
@@ -918,11 +972,14 @@ int launch(const Args& P, int ctas, cudaStream_t st) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   if (cudaLaunchKernelEx(&cfg, latent_decode_kernel<T, N>, P) != cudaSuccess) return GEMQ_ERR_LAUNCH;
-  const long long rows = static_cast<long long>(P.a.batch) * P.a.steps * P.a.heads, most = 4ll * ctas;
-  cfg.gridDim = dim3(static_cast<unsigned>(rows < most ? rows : most));
-  cfg.blockDim = dim3(kJoinThreads);
+  const long long rows = static_cast<long long>(P.a.batch) * P.a.steps * P.a.heads, most = 16ll * ctas;
+  const bool few = rows <= 2 * ctas;
+  const long long jobs = few ? rows * (P.a.rank / 128) : rows;
+  cfg.gridDim = dim3(static_cast<unsigned>(jobs < most ? jobs : most));
+  cfg.blockDim = dim3(few ? 256 : 128);
   cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, latent_join_kernel<T>, P, N, ctas) == cudaSuccess ? GEMQ_OK : GEMQ_ERR_LAUNCH;
+  const cudaError_t e = few ? cudaLaunchKernelEx(&cfg, latent_join_kernel<T, 8>, P, N, ctas) : cudaLaunchKernelEx(&cfg, latent_join_kernel<T, 1>, P, N, ctas);
+  return e == cudaSuccess ? GEMQ_OK : GEMQ_ERR_LAUNCH;
 }
 
 template <typename T>
@@ -957,6 +1014,8 @@ extern "C" int gemq_latent_decode(const gemq_latent_decode_t* A, void* scratch, 
   P.part_o = reinterpret_cast<float*>(static_cast<char*>(scratch) + s.o);
   P.slots = s.slots;
   P.scale = A->scale * kLog2e;
+  P.per = div_by(A->steps * A->heads);
+  P.heads = div_by(A->heads);
   const int rows = A->page_size < kTile ? A->page_size : kTile;
   const int blocks = A->rank / 64 + 1;
   if (!tensor_map_pages(&P.latent_map, A->cache, blocks, A->page_size, A->page_stride, A->n_pages, rows, A->page_size < kTile ? 1 : 2) ||
