@@ -104,8 +104,8 @@ __device__ __forceinline__ Entry entry_here(const Args& P, int e) {
     x.len = clamp_length(A.lens[b], A.table_pitch, A.page_size, A.err);
   }
   x.tiles = cdiv(x.len, kTile);
-  // Measured, two and more pieces of a CTA against one: 16 rows 3.4 us a piece and 2.2 a tile, 64 rows 6 us and 1.7.
-  x.piece = x.rows <= 32 ? 6 : 14;
+  // Measured, two and more pieces of a CTA against one: 16 rows 3.4 us a piece and 2.2 a tile, 64 rows 4 us and 1.7.
+  x.piece = x.rows <= 32 ? 6 : 9;
   x.cost = x.tiles ? 4 * x.tiles + x.piece : 0;
   return x;
 }
@@ -454,31 +454,39 @@ __device__ __forceinline__ void finish_piece(Smem<N>& S, const Args& P, const Pi
   if (whole) asm volatile("bar.sync 2, 128;" ::: "memory");  // the factors
   wait_for<N != 64>(&S.o_full[piece % kOs], (piece / kOs) & 1, &S.abort, A.err);
   tc_fence_after_sync();
+  // 16 rows of queries at a time, all their dimensions in flight
+  const int quarters = A.rank / 128;
 #pragma unroll 1
   for (int j = 0; j < p.rows; j += 16) {
-    float f[8];  // of the rows that the thread stores: every second one
+    uint32_t o[64];
 #pragma unroll
-    for (int x = 0; x < 8; ++x) f[x] = whole ? S.result[j + 2 * x + (lane & 1)].y : 0.f;
-#pragma unroll 1
-    for (int m = 0; m < A.rank / 128; ++m) {
-      uint32_t o[16];
-      tmem_load16(acc + lanes + m * N + j, o);
-      tmem_loaded(o);
-      if (whole) {
-        T* out = static_cast<T*>(A.out) + static_cast<long long>(p.row0 + j + (lane & 1)) * A.rank + 128 * m + (me & ~1);
+    for (int m = 0; m < 4; ++m)
+      if (m < quarters) tmem_load16(acc + lanes + m * N + j, o + 16 * m);
+    tmem_loaded(o);
+    if (whole) {
+      T* out = static_cast<T*>(A.out) + static_cast<long long>(p.row0 + j + (lane & 1)) * A.rank + (me & ~1);
 #pragma unroll
-        for (int x = 0; x < 16; x += 2) {  // an even lane takes row x of a pair of dimensions, its neighbour row x + 1
-          const float give = __uint_as_float(lane & 1 ? o[x] : o[x + 1]), keep = __uint_as_float(lane & 1 ? o[x + 1] : o[x]);
-          const float got = __shfl_xor_sync(0xffffffffu, give, 1), k = f[x >> 1];
-          const uint32_t w = lane & 1 ? Pair<T>::r(got * k, keep * k) : Pair<T>::r(keep * k, got * k);
-          if (j + x + (lane & 1) < p.rows) *reinterpret_cast<uint32_t*>(out + x * A.rank) = w;
-        }
-      } else if (slot < P.slots) {
-        float* out = P.part_o + (static_cast<long long>(slot) * N + j) * A.rank + 128 * m + me;
+      for (int x = 0; x < 16; x += 2) {  // an even lane takes row x of a pair of dimensions, its neighbour row x + 1
+        const float f = S.result[j + x + (lane & 1)].y;
+        const bool on = j + x + (lane & 1) < p.rows;
 #pragma unroll
-        for (int x = 0; x < 16; ++x)
-          if (j + x < p.rows) out[x * A.rank] = __uint_as_float(o[x]);
+        for (int m = 0; m < 4; ++m)
+          if (m < quarters) {
+            const float a = __uint_as_float(o[16 * m + x]), b = __uint_as_float(o[16 * m + x + 1]);
+            const float got = __shfl_xor_sync(0xffffffffu, lane & 1 ? a : b, 1) * f, keep = (lane & 1 ? b : a) * f;
+            if (on) *reinterpret_cast<uint32_t*>(out + 128 * m) = lane & 1 ? Pair<T>::r(got, keep) : Pair<T>::r(keep, got);
+          }
+        out += 2 * A.rank;
       }
+    } else if (slot < P.slots) {
+      float* out = P.part_o + (static_cast<long long>(slot) * N + j) * A.rank + me;
+#pragma unroll
+      for (int x = 0; x < 16; ++x, out += A.rank)
+        if (j + x < p.rows) {
+#pragma unroll
+          for (int m = 0; m < 4; ++m)
+            if (m < quarters) out[128 * m] = __uint_as_float(o[16 * m + x]);
+        }
     }
   }
   tc_fence_before_sync();
