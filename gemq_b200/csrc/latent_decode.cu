@@ -222,7 +222,9 @@ __device__ __forceinline__ void softmax_piece(Smem<N>& S, const Args& P, const P
   const bool prefix = p.e < A.groups;
   const uint32_t lanes = static_cast<uint32_t>(32 * quad) << 16;
   float ref[kCols], sum[kCols];  // what the weights refer to, their sums over the thread's positions
-  uint32_t none = ~0u;           // bit j: all scores of row j so far are -inf, the reference is 0
+  const int me = 32 * quad + lane;
+  float my_ref = 0.f;            // of row `me`
+  bool my_none = true;           // all its scores so far are -inf, the reference is 0
 #pragma unroll
   for (int j = 0; j < kCols; ++j) ref[j] = sum[j] = 0.f;
   int least = p.x.len, most = 0;
@@ -274,49 +276,47 @@ __device__ __forceinline__ void softmax_piece(Smem<N>& S, const Args& P, const P
     // the weights' place, and O, are free once the MMAs of the tile before are complete
     if (k > 0) wait_for(&S.done[(k - 1) % kSlots], ((k - 1) / kSlots) & 1, &S.abort, err);
     if (move) {
-      float top[kCols];
+      // A thread a row of queries from here: short code, as most launches come here once, with nothing of it in the instruction cache (all
+      // threads with the maxima of their rows, by shuffles: 6500 cycles for 48 rows).  The maxima meet in the place of the weights.
+      float* const scratch = reinterpret_cast<float*>(S.p);
 #pragma unroll
-      for (int j = 0; j < kCols; ++j) {
-        top[j] = fmaxf(v[2 * j], v[2 * j + 1]);
-#pragma unroll
-        for (int x = 4; x < 32; x <<= 1) top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], x));
-      }
-      if (lane < 4) {
-#pragma unroll
-        for (int j = 0; j < kCols; j += 2)
-          *reinterpret_cast<float2*>(&S.wmax[quad][4 * j + 2 * lane]) = make_float2(top[j], top[j + 1]);
-      }
+      for (int j = 0; j < kCols; j += 2)
+        *reinterpret_cast<float2*>(scratch + (8 * quad + (lane >> 2)) * NP + 4 * j + 2 * (lane & 3)) =
+            make_float2(fmaxf(v[2 * j], v[2 * j + 1]), fmaxf(v[2 * j + 2], v[2 * j + 3]));
       asm volatile("bar.sync 1, 128;" ::: "memory");
-      float f[kCols];
-      unset = false;
-#pragma unroll
-      for (int j = 0; j < kCols; ++j) {
-        const int col = 8 * (j >> 1) + 2 * (lane & 3) + (j & 1);
-#pragma unroll
-        for (int w = 0; w < 4; ++w) top[j] = fmaxf(top[j], S.wmax[w][col]);
+      bool still = false;
+      if (me < NP) {
+        float top = -INFINITY;
+#pragma unroll 4
+        for (int r = 0; r < 32; ++r) top = fmaxf(top, scratch[r * NP + me]);
         // relative to the reference so far; a row that has none takes what there is
-        const bool new_one = none >> j & 1;
-        const float up = new_one ? top[j] - kOffset : fmaxf(top[j] - kOffset, 0.f);
-        const bool still = up == -INFINITY;
-        const float by = still ? 0.f : up;
-        if (!still) none &= ~(1u << j);
-        unset |= still && S.limit[col] > 0;
-        f[j] = new_one ? 1.f : exp2_fast(-by);
-        ref[j] += by;
-        sum[j] *= f[j];
-        v[2 * j] -= by;
-        v[2 * j + 1] -= by;
+        const float up = my_none ? top - kOffset : fmaxf(top - kOffset, 0.f);
+        const bool nothing = up == -INFINITY;
+        const float by = nothing ? 0.f : up;
+        still = nothing && S.limit[me] > 0;
+        S.wmax[0][me] = by;
+        S.fac[me] = my_none ? 1.f : exp2_fast(-by);
+        my_none = my_none && nothing;
+        my_ref += by;
       }
-      unset = __any_sync(0xffffffffu, unset);
-      if (i > 0) {
-        if (lane < 4 && quad == 0) {
+      unset = any_of_softmax(still);
 #pragma unroll
-          for (int j = 0; j < kCols; j += 2) *reinterpret_cast<float2*>(&S.fac[4 * j + 2 * lane]) = make_float2(f[j], f[j + 1]);
-        }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+      for (int j = 0; j < kCols; j += 2) {
+        const float2 by = *reinterpret_cast<const float2*>(&S.wmax[0][4 * j + 2 * (lane & 3)]);
+        const float2 f = *reinterpret_cast<const float2*>(&S.fac[4 * j + 2 * (lane & 3)]);
+        ref[j] += by.x;
+        ref[j + 1] += by.y;
+        sum[j] *= f.x;
+        sum[j + 1] *= f.y;
+        v[2 * j] -= by.x;
+        v[2 * j + 1] -= by.x;
+        v[2 * j + 2] -= by.y;
+        v[2 * j + 3] -= by.y;
+      }
+      if (i > 0) {
         tc_fence_after_sync();
         for (int m = 0; m < blocks / 2; ++m)
-#pragma unroll
+#pragma unroll 1
           for (int j = 0; j < NP; j += 16) {
             uint32_t o[16];
             tmem_load16(acc + lanes + m * N + j, o);
@@ -387,20 +387,14 @@ __device__ __forceinline__ void softmax_piece(Smem<N>& S, const Args& P, const P
   for (int j = 0; j < kCols; ++j)
 #pragma unroll
     for (int x = 4; x < 32; x <<= 1) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], x);
-  asm volatile("bar.sync 1, 128;" ::: "memory");  // maxima and factors of the last correction are read
+  asm volatile("bar.sync 1, 128;" ::: "memory");  // what the last correction left there is read
   if (lane < 4) {
 #pragma unroll
-    for (int j = 0; j < kCols; j += 2) {
-      *reinterpret_cast<float2*>(&S.wmax[quad][4 * j + 2 * lane]) = make_float2(sum[j], sum[j + 1]);
-      if (quad == 0)
-        *reinterpret_cast<float2*>(&S.fac[4 * j + 2 * lane]) =
-            make_float2(none >> j & 1 ? -INFINITY : ref[j], none >> (j + 1) & 1 ? -INFINITY : ref[j + 1]);
-    }
+    for (int j = 0; j < kCols; j += 2) *reinterpret_cast<float2*>(&S.wmax[quad][4 * j + 2 * lane]) = make_float2(sum[j], sum[j + 1]);
   }
   wait_for(&S.r_free, (piece & 1) ^ 1, &S.abort, err);
   asm volatile("bar.sync 1, 128;" ::: "memory");
-  const int me = 32 * quad + lane;
-  if (me < NP) S.result[me] = make_float2(S.fac[me], S.wmax[0][me] + S.wmax[1][me] + S.wmax[2][me] + S.wmax[3][me]);
+  if (me < NP) S.result[me] = make_float2(my_none ? -INFINITY : my_ref, S.wmax[0][me] + S.wmax[1][me] + S.wmax[2][me] + S.wmax[3][me]);
   __syncwarp();
   if (lane == 0) mbar_arrive(&S.r_full);
 }
