@@ -109,7 +109,7 @@ __device__ __forceinline__ bool has_nonfinite(uint4 v) {
   return has_nonfinite<T>(v.x) || has_nonfinite<T>(v.y) || has_nonfinite<T>(v.z) || has_nonfinite<T>(v.w);
 }
 // The same in all lanes, and known to be so: what the TMA and MMA instructions take stays in uniform registers.
-__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+__device__ __forceinline__ int uniform(int v) { return static_cast<int>(__reduce_or_sync(0xffffffffu, static_cast<unsigned>(v))); }
 
 }  // namespace latent
 }  // namespace gemq

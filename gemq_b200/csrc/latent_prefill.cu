@@ -9,12 +9,14 @@
 // tiles of 128 keys: while the exponentials of one tile are formed the MMAs of the other run.  Scores, and in their place the weights
 // (16 bits), and the sums stay in tensor memory: 2 x (128 + 128) columns, all of it.
 //   warp 0      TMA: queries once, then two places of keys (48 KB) and one of values (32 KB)
-//   warp 1      MMAs: O0 of tile j, S0 of tile j + 1, O1 of tile j, S1 of tile j + 1
+//   warps 1, 2  MMAs of either tile: O of keys j, then S of keys j + 1 in its weights' place.  (One warp for both left the tensor cores idle for
+//               250 to 600 cycles between any two products.)
+//   warp 3      a second pass only, see below
 //   warps 4-7, 8-11   softmax of either tile, results
 // The reference of a row's weights moves only when its scores exceed it by 2^8; then its sums are corrected in tensor memory.
 //
 // What a query must not see is given a weight of 0.  If such a row of v holds an infinity or a NaN the product still is NaN: a block with a
-// result that is not finite is computed once more, and warps 2 and 3 set to zero, in the tiles that not all of its queries see whole, what
+// result that is not finite is computed once more, and warp 3 sets to zero, in the tiles that not all of its queries see whole, what
 // is hidden from all and what is not finite; a query that sees one of the latter gets a NaN for its weight.  Every wait is bounded.
 #include "latent.cuh"
 
@@ -39,7 +41,7 @@ struct Smem {
   alignas(1024) unsigned char q[2][3][kBlock];
   unsigned char k[2][3][kBlock];
   unsigned char v[2][kBlock];
-  alignas(8) unsigned long long q_full[2], k_full[2], k_free[2], v_full, v_free, v_clean, s_full[2], p_full[2], o_full[2];
+  alignas(8) unsigned long long q_full[2], k_full[2], k_free[2], v_full, v_free, v_clean, s_full[2], p_full[2][2], o_full[2];
   uint32_t poison[4];
   Item item;
   uint32_t tmem_base;
@@ -52,6 +54,38 @@ struct Args {
   gemq_latent_prefill_t a;
   float scale;  // times log2 e
 };
+
+// Two 32-bit numbers in a register pair: one instruction for both.
+__device__ __forceinline__ unsigned long long both(float a, float b) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void fma2(float& x, float& y, unsigned long long m, unsigned long long c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(both(x, y)), "l"(m), "l"(c));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(r));
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// A wait of the MMA warp, which stands between two products: it looks again and again (about a second in all).
+__device__ __forceinline__ void spin_for(unsigned long long* bar, uint32_t parity, int* abort, int* err) {
+  for (int i = 0; i < (1 << 25); ++i) {
+    if (mbar_test_wait(bar, parity)) return;
+    if ((i & 0xfff) == 0xfff && *reinterpret_cast<volatile int*>(abort)) return;
+  }
+  *reinterpret_cast<volatile int*>(abort) = 1;
+  atomicExch(err, GEMQ_LATENT_WAIT);
+}
 
 // Whether any thread of the CTA says so; all its threads come here.
 __device__ __forceinline__ bool any_in_cta(bool mine) {
@@ -82,14 +116,15 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __gri
     for (int i = 0; i < 2; ++i) {
       mbar_init(&S.q_full[i], 1);
       mbar_init(&S.k_full[i], 1);
-      mbar_init(&S.k_free[i], 1);
+      mbar_init(&S.k_free[i], 2);
       mbar_init(&S.s_full[i], 1);
-      mbar_init(&S.p_full[i], 4);
+      mbar_init(&S.p_full[i][0], 4);
+      mbar_init(&S.p_full[i][1], 4);
       mbar_init(&S.o_full[i], 1);
     }
     mbar_init(&S.v_full, 1);
-    mbar_init(&S.v_free, 1);
-    mbar_init(&S.v_clean, 2);
+    mbar_init(&S.v_free, 2);
+    mbar_init(&S.v_clean, 1);
     S.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -197,70 +232,78 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __gri
       // The copies in flight end before the CTA does: the MMAs waited for all of them, unless a wait ran out.
       if (*reinterpret_cast<volatile int*>(&S.abort))
         for (int i = 0; i < 2000; ++i) __nanosleep(1000);
-    } else if (warp == 1) {
+    } else if (warp < 3) {
+      const int t = warp - 1, mine = tiles[t];
       const uint32_t idesc_s = umma_idesc_f16(Pair<T>::kBf16, kRows, kRows), idesc_o = umma_idesc_f16(Pair<T>::kBf16, kRows, kValue) | kUmmaTransposeB;
-      const uint64_t q = umma_desc_k_sw128(smem_u32(S.q[0][0])), k = umma_desc_k_sw128(smem_u32(S.k[0][0])),
+      const uint64_t q = umma_desc_k_sw128(smem_u32(S.q[t][0])), k = umma_desc_k_sw128(smem_u32(S.k[0][0])),
                      v = umma_desc_mn_sw128(smem_u32(S.v[0]), kBlock);
+      const uint32_t s_at = tmem + t * kRows, o_at = tmem + 2 * kRows + t * kValue;
+      if (mine > 0) wait_for(&S.q_full[t], 0, &S.abort, err);
       for (int pass = 0;; ++pass) {
-        auto scores = [&](int t, int j) {
+        // S of keys j; a place of keys, and that of the values, is free when both tiles are done with it or have no use for it
+        auto scores = [&](int j) {
           const int s = j & 1;
-          wait_for(&S.k_full[s], (pass * k_uses[s] + (j >> 1)) & 1, &S.abort, err);
-          tc_fence_after_sync();
-          const uint64_t a = q + t * (3 * kBlock >> 4), b = k + s * (3 * kBlock >> 4);
-          if (elect_lane()) {
+          spin_for(&S.k_full[s], (pass * k_uses[s] + (j >> 1)) & 1, &S.abort, err);
+          if (j < mine) {
+            tc_fence_after_sync();
+            const uint64_t b = k + s * (3 * kBlock >> 4);
+            if (elect_lane()) {
 #pragma unroll
-            for (int i = 0; i < 12; ++i)
-              umma_ss_f16(tmem + t * kRows, a + (i >> 2) * (kBlock >> 4) + (i & 3) * 2, b + (i >> 2) * (kBlock >> 4) + (i & 3) * 2, idesc_s, i != 0);
-            umma_commit(&S.s_full[t]);
-            if (t == 1 || j >= tiles[1]) umma_commit(&S.k_free[s]);
+              for (int i = 0; i < 12; ++i)
+                umma_ss_f16(s_at, q + (i >> 2) * (kBlock >> 4) + (i & 3) * 2, b + (i >> 2) * (kBlock >> 4) + (i & 3) * 2, idesc_s, i != 0);
+              umma_commit(&S.s_full[t]);
+              umma_commit(&S.k_free[s]);
+            }
+          } else if (elect_lane()) {
+            mbar_arrive(&S.k_free[s]);
           }
           __syncwarp();
         };
-        auto sums = [&](int t, int j) {
-          wait_for(&S.p_full[t], (pass * tiles[t] + j) & 1, &S.abort, err);
-          wait_for(pass ? &S.v_clean : &S.v_full, j & 1, &S.abort, err);
-          tc_fence_after_sync();
-          const uint32_t o = tmem + 2 * kRows + t * kValue, p = tmem + t * kRows;
-          if (elect_lane()) {
+        if (most > 0) scores(0);
+        for (int j = 0; j < most; ++j) {
+          if (j < mine) {  // by the halves of the weights: the first is multiplied while the second is formed
+            spin_for(&S.p_full[t][0], (pass * mine + j) & 1, &S.abort, err);
+            spin_for(pass ? &S.v_clean : &S.v_full, j & 1, &S.abort, err);
+            tc_fence_after_sync();
+            if (elect_lane()) {
 #pragma unroll
-            for (int i = 0; i < kRows / 16; ++i) umma_ts_f16_one(o, p + i * 8, v + i * (2048 >> 4), idesc_o, j != 0 || i != 0);
-            if (t == 1 || j >= tiles[1]) umma_commit(&S.v_free);
-            if (j == tiles[t] - 1) umma_commit(&S.o_full[t]);
+              for (int i = 0; i < kRows / 32; ++i) umma_ts_f16_one(o_at, s_at + i * 8, v + i * (2048 >> 4), idesc_o, j != 0 || i != 0);
+            }
+            __syncwarp();
+            spin_for(&S.p_full[t][1], (pass * mine + j) & 1, &S.abort, err);
+            tc_fence_after_sync();
+            if (elect_lane()) {
+#pragma unroll
+              for (int i = kRows / 32; i < kRows / 16; ++i) umma_ts_f16_one(o_at, s_at + i * 8, v + i * (2048 >> 4), idesc_o, 1);
+              umma_commit(&S.v_free);
+              if (j == mine - 1) umma_commit(&S.o_full[t]);
+            }
+          } else {
+            spin_for(&S.v_full, (pass * most + j) & 1, &S.abort, err);
+            if (elect_lane()) mbar_arrive(&S.v_free);
           }
           __syncwarp();
-        };
-        for (int t = 0; t < 2; ++t)
-          if (tiles[t] > 0) {
-            wait_for(&S.q_full[t], 0, &S.abort, err);
-            scores(t, 0);
-          }
-        for (int j = 0; j < most; ++j)
-          for (int t = 0; t < 2; ++t) {
-            if (j < tiles[t]) sums(t, j);
-            if (j + 1 < tiles[t]) scores(t, j + 1);
-          }
+          if (j + 1 < most) scores(j + 1);
+        }
         if (!any_in_cta(false) || pass == 1) break;
       }
     } else if (any_in_cta(false)) {
-      // second pass: a warp has 64 rows of a tile of v
-      const int r0 = (warp - 2) * 64;
       for (int j = 0; j < most; ++j) {
         wait_for(&S.v_full, (most + j) & 1, &S.abort, err);
-        uint32_t poison[2] = {0, 0};
-        for (int r = max(least_of_all - j * kRows - r0, 0); r < 64; ++r) {
-          uint2* at = reinterpret_cast<uint2*>(S.v[lane >> 4] + (r0 + r) * 128) + (lane & 15);
-          bool wipe = j * kRows + r0 + r >= most_of_all;
-          if (!wipe) {
-            const uint2 x = *at;
-            wipe = __any_sync(0xffffffffu, has_nonfinite<T>(x.x) || has_nonfinite<T>(x.y));
-            if (wipe) poison[r >> 5] |= 1u << (r & 31);
+        uint32_t poison[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          for (int r = max(least_of_all - j * kRows - 32 * w, 0); r < 32; ++r) {
+            uint2* at = reinterpret_cast<uint2*>(S.v[lane >> 4] + (32 * w + r) * 128) + (lane & 15);
+            bool wipe = j * kRows + 32 * w + r >= most_of_all;
+            if (!wipe) {
+              const uint2 x = *at;
+              wipe = __any_sync(0xffffffffu, has_nonfinite<T>(x.x) || has_nonfinite<T>(x.y));
+              if (wipe) poison[w] |= 1u << r;
+            }
+            if (wipe) *at = make_uint2(0, 0);
           }
-          if (wipe) *at = make_uint2(0, 0);
-        }
-        if (lane == 0) {
-          S.poison[2 * (warp - 2)] = poison[0];
-          S.poison[2 * (warp - 2) + 1] = poison[1];
-        }
+        if (lane < 4) S.poison[lane] = lane == 0 ? poison[0] : lane == 1 ? poison[1] : lane == 2 ? poison[2] : poison[3];
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&S.v_clean);
@@ -283,8 +326,11 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __gri
         for (int c = 0; c < 4; ++c) tmem_load32(s + 32 * c, raw + 32 * c);
         tmem_loaded(raw);
         float* v = reinterpret_cast<float*>(raw);
+        {
+          const unsigned long long m = both(P.scale, P.scale), c2 = both(-ref, -ref);
 #pragma unroll
-        for (int c = 0; c < kRows; ++c) v[c] = fmaf(v[c], P.scale, -ref);
+          for (int c = 0; c < kRows; c += 2) fma2(v[c], v[c + 1], m, c2);
+        }
         if (pass) {
           wait_for(&S.v_clean, j & 1, &S.abort, err);
 #pragma unroll
@@ -297,9 +343,10 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __gri
           for (int c = 0; c < kRows; ++c)
             if (c >= here) v[c] = -INFINITY;
         }
-        float top = fmaxf(v[0], v[1]);
+        float most4[4] = {v[0], v[1], v[2], v[3]};  // four chains
 #pragma unroll
-        for (int c = 2; c < kRows; c += 2) top = fmaxf(top, fmaxf(v[c], v[c + 1]));
+        for (int c = 4; c + 1 < kRows; c += 2) most4[(c >> 1) & 3] = max3(most4[(c >> 1) & 3], v[c], v[c + 1]);
+        const float top = fmaxf(fmaxf(most4[0], most4[1]), fmaxf(most4[2], most4[3]));
         if (__any_sync(0xffffffffu, none ? top > -INFINITY : top > kOffset + 8.f)) {
           const float up = none ? top - kOffset : fmaxf(top - kOffset, 0.f), by = up == -INFINITY ? 0.f : up;
           const float f = none ? 1.f : exp2_fast(-by);
@@ -320,23 +367,27 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __gri
             }
           }
         }
-        float part[4] = {0.f, 0.f, 0.f, 0.f};
+        unsigned long long part[2] = {0, 0};  // sums of the even and the odd keys, twice
 #pragma unroll
         for (int c = 0; c < kRows; c += 32) {
           uint32_t w[16];
 #pragma unroll
           for (int y = 0; y < 16; ++y) {
             const float a = exp2_fast(v[c + 2 * y]), b = exp2_fast(v[c + 2 * y + 1]);
-            part[y & 3] += a + b;
+            part[y & 1] = add2(part[y & 1], both(a, b));
             w[y] = Pair<T>::r(a, b);
           }
           tmem_store16(s + c / 2, w);
+          if (c & 32) {  // a half is there
+            tmem_stored();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&S.p_full[t][c >> 6]);
+          }
         }
-        sum += (part[0] + part[1]) + (part[2] + part[3]);
-        tmem_stored();
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&S.p_full[t]);
+        float even, odd;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(even), "=f"(odd) : "l"(add2(part[0], part[1])));
+        sum += even + odd;
       }
       bool bad = false;
       if (t * kRows + 32 * quad < rows) {  // the warp has rows
