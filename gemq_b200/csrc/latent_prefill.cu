@@ -71,6 +71,12 @@ __device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigne
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+// Stays where it stands among the stores and hand-overs: those of the second half are not to be formed ahead of the first half's.
+__device__ __forceinline__ float exp2_here(float x) {
+  float y;
+  asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -143,12 +149,14 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __gri
         k0 = within(A.cu_k[b], A.k_rows);
         keys = b < A.batch ? max(within(A.cu_k[b + 1], A.k_rows) - k0, 0) : 0;
       }
+      // Those of many keys first (of 32 sequences at a time): what begins last should be short.
       const int mine = n > 0 ? cdiv(n, 2 * kRows) : 0;
-      int upto = mine;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, upto, d);
-        if (lane >= d) upto += v;
+      int upto = mine, all = mine;
+#pragma unroll 4
+      for (int d = 1; d < 32; ++d) {
+        const int who = (lane + d) & 31, k = __shfl_sync(0xffffffffu, keys, who), m = __shfl_sync(0xffffffffu, mine, who);
+        all += m;
+        if (k > keys || (k == keys && who < lane)) upto += m;
       }
       const bool hit = at >= seen + upto - mine && at < seen + upto;
       if (hit) {
@@ -156,7 +164,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __gri
         S.item = {q0 + r0, min(n - r0, 2 * kRows), k0, keys, A.causal ? r0 + 1 + keys - n : kAllKeys};
       }
       found = __any_sync(0xffffffffu, hit);
-      seen += __shfl_sync(0xffffffffu, upto, 31);
+      seen += all;
     }
     if (!found && lane == 0) S.item = {0, 0, 0, 0, 0};
   }
@@ -373,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __gri
           uint32_t w[16];
 #pragma unroll
           for (int y = 0; y < 16; ++y) {
-            const float a = exp2_fast(v[c + 2 * y]), b = exp2_fast(v[c + 2 * y + 1]);
+            const float a = exp2_here(v[c + 2 * y]), b = exp2_here(v[c + 2 * y + 1]);
             part[y & 1] = add2(part[y & 1], both(a, b));
             w[y] = Pair<T>::r(a, b);
           }
@@ -400,19 +408,21 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __gri
           const float f = limit > 0 ? 1.f / sum : 0.f;
           float check = 0.f;
 #pragma unroll 1
-          for (int c = 0; c < kValue; c += 16) {
-            uint32_t x[16], w[8];
-            tmem_load16(o + c, x);
+          for (int c = 0; c < kValue; c += 64) {
+            uint32_t x[64];
+            tmem_load32(o + c, x);
+            tmem_load32(o + c + 32, x + 32);
             tmem_loaded(x);
 #pragma unroll
-            for (int y = 0; y < 8; ++y) {
-              const float a = __uint_as_float(x[2 * y]) * f, b = __uint_as_float(x[2 * y + 1]) * f;
-              check += (a - a) + (b - b);  // 0, or NaN
-              w[y] = Pair<T>::r(a, b);
-            }
-            if (on) {
-              reinterpret_cast<uint4*>(to + c)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-              reinterpret_cast<uint4*>(to + c)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+            for (int y = 0; y < 64; y += 8) {
+              uint32_t w[4];
+#pragma unroll
+              for (int z = 0; z < 4; ++z) {
+                const float a = __uint_as_float(x[y + 2 * z]) * f, b = __uint_as_float(x[y + 2 * z + 1]) * f;
+                check += (a - a) + (b - b);  // 0, or NaN
+                w[z] = Pair<T>::r(a, b);
+              }
+              if (on) *reinterpret_cast<uint4*>(to + c + y) = make_uint4(w[0], w[1], w[2], w[3]);
             }
           }
           bad = on && check != 0.f;
