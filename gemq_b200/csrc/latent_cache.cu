@@ -52,6 +52,15 @@ __global__ void __launch_bounds__(32 * kAppendWarps) latent_append_kernel(const 
   for (int i = 0; i < 2; ++i) v[i] = lane + 32 * i < pieces ? src[lane + 32 * i] : make_uint4(0, 0, 0, 0);
   const uint32_t kp = reinterpret_cast<const uint32_t*>(src + pieces)[lane];
 
+  // the first 16 heads' queries are asked for here: eight lanes a head, four pairs a lane
+  const T* q = static_cast<const T*>(P.q) + t * P.q_token + (lane & 7) * 8;
+  uint4 early[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int h = (lane >> 3) + 4 * i;
+    if (h < P.heads) early[i] = *reinterpret_cast<const uint4*>(q + h * P.q_head);
+  }
+
   const double turns = static_cast<double>(P.positions[t]) * static_cast<double>(P.inv_freq[lane]) * 0.15915494309189535;  // 1 / 2 pi
   float sn, cs;
   sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &sn, &cs);
@@ -101,18 +110,14 @@ __global__ void __launch_bounds__(32 * kAppendWarps) latent_append_kernel(const 
     reinterpret_cast<uint32_t*>(row + pieces)[lane] = o;
     if (stored) reinterpret_cast<uint32_t*>(stored + pieces)[lane] = o;
   }
-  // queries: eight lanes a head, four pairs a lane
   float c4[4], s4[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     c4[k] = __shfl_sync(0xffffffffu, cs, (lane & 7) * 4 + k);
     s4[k] = __shfl_sync(0xffffffffu, sn, (lane & 7) * 4 + k);
   }
-  const T* q = static_cast<const T*>(P.q) + t * P.q_token + (lane & 7) * 8;
   T* qo = static_cast<T*>(P.q_out) + static_cast<long long>(t) * P.heads * kRope + (lane & 7) * 8;
-#pragma unroll 4
-  for (int h = lane >> 3; h < P.heads; h += 4) {
-    const uint4 x = *reinterpret_cast<const uint4*>(q + h * P.q_head);
+  auto turn = [&](int h, const uint4& x) {
     uint4 o;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -120,7 +125,14 @@ __global__ void __launch_bounds__(32 * kAppendWarps) latent_append_kernel(const 
       reinterpret_cast<uint32_t*>(&o)[k] = Pair<T>::r(f.x * c4[k] - f.y * s4[k], f.x * s4[k] + f.y * c4[k]);
     }
     *reinterpret_cast<uint4*>(qo + h * kRope) = o;
+  };
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int h = (lane >> 3) + 4 * i;
+    if (h < P.heads) turn(h, early[i]);
   }
+#pragma unroll 4
+  for (int h = (lane >> 3) + 16; h < P.heads; h += 4) turn(h, *reinterpret_cast<const uint4*>(q + h * P.q_head));
 }
 
 // A CTA copies 16 KB of a page of one layer at a time, four 16-byte loads a thread in flight.
