@@ -203,6 +203,7 @@ int64_t cache_rank(const Tensor* c, const Tensor& like, int64_t* page_stride) {
   const int64_t pages = c->size(0), page = c->size(1), rank = c->size(2) - 64;
   int64_t s[2];
   if (rank < 128 || rank > 512 || rank % 128 || pages <= 0 || pages * page >= (int64_t(1) << 31) || c->stride(1) != c->size(2)) return 0;
+  if (pages > 1 && c->stride(0) < page * c->size(2)) return 0;
   if (!(page == 16 || page == 32 || (page > 0 && page % 64 == 0)) || !row_strides(*c, s)) return 0;
   *page_stride = s[0];
   return rank;

@@ -128,6 +128,10 @@ struct Cut {
   }
 };
 
+// Where a piece of row tile rt leaves its sums.  With prefixes each does, and pieces of the launch in order grow by their row tile or their
+// CTA.  Without, a CTA has two such pieces at most: the end of a row tile that others began, and one that others go on with.
+__device__ __forceinline__ int slot_of(bool groups, int rt, int cta, bool last) { return groups ? rt + cta : 2 * cta + (last ? 0 : 1); }
+
 struct Piece {
   Entry x;
   int e, t0, n;      // entry, first tile, tiles
@@ -135,6 +139,7 @@ struct Piece {
   int rt;            // row tile of the launch
   __device__ __forceinline__ int width() const { return (rows + 15) & ~15; }
   __device__ __forceinline__ bool whole() const { return n == x.tiles; }
+  __device__ __forceinline__ bool last() const { return t0 + n == x.tiles; }
 };
 
 template <int N, bool CALL = true>
@@ -432,7 +437,7 @@ __device__ __forceinline__ void finish_piece(Smem<N>& S, const Args& P, const Pi
   const int lane = threadIdx.x & 31, quad = (threadIdx.x >> 5) & 3, me = 32 * quad + lane;
   const uint32_t lanes = static_cast<uint32_t>(32 * quad) << 16;
   const bool prefix = p.e < A.groups, whole = p.whole() && A.groups == 0;
-  const int slot = p.rt + static_cast<int>(blockIdx.x);  // pieces of the launch in order: either grows
+  const int slot = slot_of(A.groups > 0, p.rt, blockIdx.x, p.last());
   if (slot >= P.slots) atomicExch(A.err, GEMQ_LATENT_BAD_LENGTH);
   wait_for<N != 64>(&S.r_full, piece & 1, &S.abort, A.err);
   if (me < p.rows && (whole || slot < P.slots)) {
@@ -833,14 +838,15 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) latent_join_kernel(cons
       waited = true;
     }
     const Cut cut(P.ctl[0], sms);
-    int slot[2] = {0, 0}, count[2] = {0, 0}, at[2] = {0, 0};  // runs of slots: of the group's prefix, of the sequence's own tiles
+    int rt[2] = {0, 0}, first[2] = {0, 0}, count[2] = {0, 0}, at[2] = {0, 0};  // runs of pieces: of the group's prefix, of the sequence's own tiles
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const int e = k ? A.groups + b : g;
       if (x[k].tiles > 0) {
         const int r = row - x[k].row0, base = P.ctl[2 + 2 * e] + r / N * x[k].cost;
         const int c0 = cut.cta_of(base + x[k].piece), c1 = cut.cta_of(base + x[k].piece + 4 * (x[k].tiles - 1));
-        slot[k] = P.ctl[3 + 2 * e] + r / N + c0;
+        rt[k] = P.ctl[3 + 2 * e] + r / N;
+        first[k] = c0;
         count[k] = c1 - c0 + 1;
         at[k] = r % N;
       }
@@ -855,7 +861,9 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) latent_join_kernel(cons
       float2 ml[kJoinAhead];
 #pragma unroll
       for (int k = 0; k < kJoinAhead; ++k) {
-        const int i = i0 + W * k, s = i < count[0] ? slot[0] + i : slot[1] + i - count[0];
+        const int i = i0 + W * k;
+        const int s = i < count[0] ? slot_of(true, rt[0], first[0] + i, false)
+                                   : slot_of(A.groups > 0, rt[1], first[1] + i - count[0], i == pieces - 1);
         ml[k] = make_float2(-INFINITY, 0.f);
         v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (i < pieces && s < P.slots) {
@@ -929,6 +937,7 @@ int check(const gemq_latent_decode_t* A) {
     return GEMQ_ERR_ALIGN;
   for (int i = 0; i < 3; ++i)
     if ((A->q_latent_stride[i] | A->q_rope_stride[i]) & 7) return GEMQ_ERR_ALIGN;
+  if (A->n_pages > 1 && A->page_stride < static_cast<int64_t>(A->page_size) * (A->rank + kRope)) return GEMQ_ERR_BAD_SHAPE;
   return GEMQ_OK;
 }
 
@@ -944,7 +953,7 @@ Scratch scratch_of(const gemq_latent_decode_t* A) {
   Scratch s;
   long long rts = static_cast<long long>(A->batch) * ((per + N - 1) / N);
   if (A->groups) rts += per * A->batch / N + A->groups;
-  s.slots = static_cast<int>(rts + sm_count_or_default());
+  s.slots = static_cast<int>(A->groups ? rts + sm_count_or_default() : 2 * sm_count_or_default());
   s.ctl = 0;
   s.ml = (sizeof(int) * (2 + 2 * (static_cast<size_t>(A->groups) + A->batch)) + 255) & ~size_t(255);
   s.o = (s.ml + sizeof(float2) * s.slots * N + 255) & ~size_t(255);

@@ -8,7 +8,8 @@ A token is cached as one row of ``rank + 64`` numbers that all heads share: the 
 of the key.  A cache is ``[pages, page_size, rank + 64]``, fp16 or bf16, any stride between pages; ``page_size`` is 16, 32 or a
 multiple of 64, ``rank`` 128, 256, 384 or 512.  Lengths, page tables and slots are device tensors that no call reads on the host,
 so every call can be captured in a CUDA graph.  Entries out of range are reported in the device's error word
-(``gemq_b200.kernels.latent_error``) and never used as an index.  Serving only: the operators have no gradients.
+(``gemq_b200.kernels.latent_error``) and never used as an index.  That word is made by the first call on a device, which belongs
+outside a capture.  Serving only: the operators have no gradients.
 """
 from __future__ import annotations
 
@@ -80,7 +81,7 @@ def _check_cache(cache: Tensor, dtype: torch.dtype):
     require(rank in (128, 256, 384, 512), f"latent rank must be 128, 256, 384 or 512, not {rank}")
     require(page in (16, 32) or (page > 0 and page % 64 == 0), f"page size must be 16, 32 or a multiple of 64, not {page}")
     require(pages > 0 and pages * page < 2 ** 31, "a cache has 1 to 2^31 - 1 rows")
-    require(cache.stride(1) == width, "the rows of a page must lie one behind the other")
+    require(cache.stride(1) == width and (pages == 1 or cache.stride(0) >= page * width), "the rows of a page must lie one behind the other, pages apart")
     return rank, _strides("cache", cache)[0]
 
 

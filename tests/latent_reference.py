@@ -20,7 +20,7 @@ def attend(q, keys, values, limits, scale):
         lse[rows] = torch.logsumexp(s, 1)
         p = torch.softmax(s, 1)
         out[rows], mass[rows] = p @ values[:limit], p @ values[:limit].abs()
-        size[rows] = (q[rows].abs() @ keys[:limit].abs().T * scale).amax(1)
+        size[rows] = (q[rows].abs() @ keys[:limit].abs().T * abs(scale)).amax(1)
     return out, lse, mass, size
 
 

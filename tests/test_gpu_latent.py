@@ -57,6 +57,8 @@ DECODE = [
     ([20000], 1, 1, 512, 64),
     ([130] * 70, 1, 16, 512, 64),
     ([1 + 37 * i % 400 for i in range(200)], 1, 4, 128, 16),
+    ([i % 3 * 50 for i in range(1000)], 1, 3, 128, 64),      # more sequences than threads
+    ([130, 45], 40, 16, 256, 32),                            # a piece of a prompt: 640 rows a sequence, some that see nothing
 ]
 
 
@@ -112,6 +114,73 @@ def test_decode_sees_nothing_behind_its_position(S, n, value):
     assert torch.equal(got[0, blind], want[0, blind]) and torch.equal(lse[0, blind], want_lse[0, blind])
     if math.isnan(value):
         assert bool(got[0, seeing].isnan().all())
+
+
+def test_decode_without_a_row():
+    """No sequence has one, in a table with and without room."""
+    from gemq_b200.kernels import latent_decode
+    for width in (0, 3):
+        cache = torch.full((4, 64, 576), NAN, dtype=torch.float16, device="cuda")
+        table = torch.full((2, width), 99, dtype=torch.int32, device="cuda")
+        q = torch.ones(2, 2, 16, 512, dtype=torch.float16, device="cuda")
+        out, lse = latent_decode(q, q[..., :64], cache, table, torch.zeros(2, dtype=torch.int32, device="cuda"), 0.1)
+        assert not bool(out.any()) and bool((lse == -INF).all())
+    out, lse = latent_decode(q[:0], q[:0, ..., :64], cache, table[:0], torch.zeros(0, dtype=torch.int32, device="cuda"), 0.1)
+    assert out.shape == (0, 2, 16, 512) and lse.shape == (0, 2, 16)
+
+
+@pytest.mark.parametrize("value", [NAN, INF])
+def test_a_querys_nan_is_its_own(value):
+    from gemq_b200.kernels import latent_decode, latent_prefill
+    q_latent, q_rope, cache, table, lens, _ = decode_case([700, 90], 2, 16, 512, 64, torch.bfloat16)
+    want = latent_decode(q_latent, q_rope, cache, table, lens, 0.07)
+    bad = q_latent.clone()
+    bad[0, 1, 5, 3] = value
+    got = latent_decode(bad, q_rope, cache, table, lens, 0.07)
+    keep = torch.ones(2, 2, 16, dtype=torch.bool, device="cuda")
+    keep[0, 1, 5] = False
+    assert all(torch.equal(a[keep], b[keep]) for a, b in zip(got, want)) and bool(got[0][0, 1, 5].isnan().all())
+    q, kv, k_rope, cu_q, cu_k = prefill_case([(300, 400)], 2, torch.bfloat16)
+    want = latent_prefill(q[..., :NOPE], q[..., NOPE:], kv, k_rope, cu_q, cu_k, 0.07)
+    bad = q.clone()
+    bad[140, 1, 7] = value
+    got = latent_prefill(bad[..., :NOPE], bad[..., NOPE:], kv, k_rope, cu_q, cu_k, 0.07)
+    keep = torch.ones(300, 2, dtype=torch.bool, device="cuda")
+    keep[140, 1] = False
+    assert all(torch.equal(a[keep], b[keep]) for a, b in zip(got, want)) and bool(got[0][140, 1].isnan().all())
+
+
+@pytest.mark.parametrize("scale", [-0.05, 0.0, 3.0])
+def test_scales(scale):
+    from gemq_b200.kernels import latent_decode, latent_prefill
+    q_latent, q_rope, cache, table, lens, rows = decode_case([200, 65], 1, 16, 512, 64, torch.float16)
+    got, lse = latent_decode(q_latent, q_rope, cache, table, lens, scale)
+    check_decode(got, lse, q_latent, q_rope, [rows_of(cache, r) for r in rows], scale)
+    q, kv, k_rope, cu_q, cu_k = prefill_case([(150, 150)], 2, torch.float16)
+    got, lse = latent_prefill(q[..., :NOPE], q[..., NOPE:], kv, k_rope, cu_q, cu_k, scale)
+    check_prefill(got, lse, [(150, 150)], q, kv, k_rope, scale, True)
+
+
+def test_prefill_without_a_key():
+    from gemq_b200.kernels import latent_prefill
+    q, kv, k_rope, cu_q, cu_k = prefill_case([(150, 0), (3, 0)], 2, torch.float16)
+    for causal in (True, False):
+        out, lse = latent_prefill(q[..., :NOPE], q[..., NOPE:], kv, k_rope, cu_q, cu_k, 0.1, causal)
+        assert not bool(out.any()) and bool((lse == -INF).all())
+    q, kv, k_rope, cu_q, cu_k = prefill_case([(0, 5)], 2, torch.float16)
+    assert latent_prefill(q[..., :NOPE], q[..., NOPE:], kv, k_rope, cu_q, cu_k, 0.1)[0].shape == (0, 2, 128)
+    q, kv, k_rope, cu_q, cu_k = prefill_case([], 2, torch.float16, spare=4)  # rows, but no sequences
+    out, lse = latent_prefill(q[..., :NOPE], q[..., NOPE:], kv, k_rope, cu_q, cu_k, 0.1)
+    assert not bool(out.any()) and bool((lse == -INF).all())
+
+
+def test_prefill_of_expanded_tensors():
+    """One query head and one key head seen as several (strides of 0)."""
+    from gemq_b200.kernels import latent_prefill
+    q, kv, k_rope, cu_q, cu_k = prefill_case([(90, 130)], 1, torch.float16)
+    want = latent_prefill(q[..., :NOPE], q[..., NOPE:], kv, k_rope, cu_q, cu_k, 0.07)
+    got = latent_prefill(q[..., :NOPE].expand(-1, 3, -1), q[..., NOPE:].expand(-1, 3, -1), kv.expand(-1, 3, -1), k_rope, cu_q, cu_k, 0.07)
+    assert all(torch.equal(a.expand(b.shape) if a.dim() == 3 else a.expand(-1, 3), b) for a, b in zip(want, got))
 
 
 def test_decode_takes_any_strides():
@@ -289,7 +358,7 @@ def masked(q, keys, values, limits, scale):
     s = (q @ keys.T * scale).masked_fill(hidden, -INF)
     lse = torch.logsumexp(s, 1)
     p = torch.exp(s - lse.clamp(min=-1e300)[:, None]).masked_fill(hidden, 0.0)
-    size = (q.abs() @ keys.abs().T * scale).masked_fill(hidden, 0.0).amax(1)
+    size = (q.abs() @ keys.abs().T * abs(scale)).masked_fill(hidden, 0.0).amax(1)
     return p @ values, lse, p @ values.abs(), size
 
 

@@ -144,6 +144,51 @@ def test_a_decode_step_captured_and_replayed():
             assert float((out.double() - want).norm() / want.norm()) < (4 + 5 * (1 + 2 * 3)) * eps / 2
 
 
+def test_every_operator_captured():
+    """Each in a graph of its own, made one after the other and replayed interleaved with eager calls on other data."""
+    from gemq_b200 import kernels as K
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    r = lambda *shape: torch.randn(*shape, device="cuda", generator=gen).half()  # noqa: E731
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    cache, table = r(40, 64, 576), torch.randperm(40, device="cuda", generator=gen).to(torch.int32)[:32].view(2, 16)
+    ql, qr, lens = r(2, 1, 16, 512), r(2, 1, 16, 64), i32(900, 70)
+    prefix, plens, starts = table[:1, :3].contiguous(), i32(150), i32(0, 2)
+    q, kv, kr, cq, ck = r(300, 4, 192), r(300, 4, 256), r(300, 64), i32(0, 100, 300), i32(0, 100, 300)
+    rows, w, inv = r(5, 576), r(512), torch.ones(32, device="cuda")
+    pos, slots = torch.arange(5, device="cuda"), torch.tensor([2400, -1, 2401, 2402, 2500], device="cuda")
+    src, dst = torch.tensor([1, 2], device="cuda"), torch.tensor([38, 39], device="cuda")
+    calls = dict(decode=lambda: K.latent_decode(ql, qr, cache, table, lens, 0.07),
+                 shared=lambda: K.latent_decode_shared(ql, qr, cache, table, lens, prefix, plens, starts, 0.07),
+                 prefill=lambda: K.latent_prefill(q[..., :128], q[..., 128:], kv, kr, cq, ck, 0.07),
+                 append=lambda: K.latent_append(rows, qr.expand(2, 5, 16, 64)[0], w, 1e-6, inv, pos, slots, cache),
+                 copy=lambda: K.copy_pages(cache, src, dst))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graphs = {}
+    with torch.cuda.stream(side):
+        for name, call in calls.items():
+            call()
+        torch.cuda.synchronize()
+        for name, call in calls.items():
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                graphs[name] = (call(), g)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for t in (ql, qr, q, kv, kr, rows):
+            t.copy_(torch.randn(t.shape, device="cuda", generator=gen))
+        for name in ("append", "copy", "decode", "prefill", "shared"):
+            out, g = graphs[name]
+            before = cache.clone()
+            g.replay()
+            after = cache.clone()
+            cache.copy_(before)
+            want = calls[name]()
+            assert torch.equal(cache, after), name
+            if out is not None:
+                assert all(torch.equal(a, b) for a, b in zip(out, want)), name
+
+
 def test_calls_on_several_streams_at_once():
     from gemq_b200 import kernels as K
     gen = torch.Generator(device="cuda").manual_seed(4)

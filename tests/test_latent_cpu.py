@@ -69,6 +69,7 @@ BAD = [
     (L.latent_decode, decode_args, dict(cache=torch.zeros(7, 64, R + 64, dtype=bf16)), "cache must be"),
     (L.latent_decode, decode_args, dict(cache=torch.zeros(0, 64, R + 64, dtype=f16)), "rows"),
     (L.latent_decode, decode_args, dict(cache=torch.zeros(7, 64, R + 128, dtype=f16)[..., :R + 64]), "one behind the other"),
+    (L.latent_decode, decode_args, dict(cache=torch.zeros(1, 64, R + 64, dtype=f16).expand(7, -1, -1)), "pages apart"),
     (L.latent_decode, decode_args, dict(q_latent=torch.zeros(B, S, H, 128, dtype=f16)), "q_latent"),
     (L.latent_decode, decode_args, dict(q_latent=torch.zeros(B, 0, H, R, dtype=f16), q_rope=torch.zeros(B, 0, H, 64, dtype=f16)), "a step and a head"),
     (L.latent_decode, decode_args, dict(q_latent=NARROW), "16-byte"),
@@ -133,7 +134,7 @@ def test_library_refuses():
 
     assert code() == -3  # no workspace
     for over, want in ((dict(rank=192), -2), (dict(rank=1024), -2), (dict(page_size=8), -2), (dict(page_size=96), -2), (dict(heads=0), -1),
-                       (dict(out=None), -1), (dict(q_latent=p + 8), -5), (dict(page_stride=4), -5), (dict(groups=1), -1),
+                       (dict(out=None), -1), (dict(q_latent=p + 8), -5), (dict(page_stride=4), -5), (dict(page_stride=0), -2), (dict(groups=1), -1),
                        (dict(batch=1 << 20, steps=1 << 10, heads=128), -2), (dict(table_pitch=1 << 30), -2), (dict(batch=-1), -1)):
         assert code(**over) == want, over
     assert code(batch=0) == 0
