@@ -108,6 +108,10 @@ template <typename T>
 __device__ __forceinline__ bool has_nonfinite(uint4 v) {
   return has_nonfinite<T>(v.x) || has_nonfinite<T>(v.y) || has_nonfinite<T>(v.z) || has_nonfinite<T>(v.w);
 }
+// A map is a launch parameter: its first use finds it in the cache.
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<unsigned long long>(map)) : "memory");
+}
 // The same in all lanes, and known to be so: what the TMA and MMA instructions take stays in uniform registers.
 __device__ __forceinline__ int uniform(int v) { return static_cast<int>(__reduce_or_sync(0xffffffffu, static_cast<unsigned>(v))); }
 

@@ -420,7 +420,9 @@ __device__ __forceinline__ void load_queries(Smem<N>& S, const Args& P, const Pi
     const uint32_t dst = smem_u32(S.q[0]) + r * 128 + (((tid & 7) ^ (r & 7)) << 4), bytes = r < p.rows ? 16 : 0;  // 0: zeros
     for (int d = 0; d <= blocks; ++d) {
       const uint4* src = d < blocks ? ql + d * 8 + (tid & 7) : qr + (tid & 7);
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + d * (N * 128)), "l"(bytes ? static_cast<const void*>(src) : A.q_latent), "r"(bytes) : "memory");
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + d * (N * 128)),
+                   "l"(bytes ? static_cast<const void*>(src) : A.q_latent), "r"(bytes)
+                   : "memory");
     }
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
@@ -496,6 +498,207 @@ __device__ __forceinline__ void finish_piece(Smem<N>& S, const Args& P, const Pi
   }
 }
 
+// ---- the warps that feed: tiles by TMA, the two products -----------------------------------------------
+template <int N>
+__device__ __forceinline__ void load_tiles(Smem<N>& S, const Args& P, const Start& start) {
+  constexpr int kLatent = Ring<N>::kLatent, kRopes = Ring<N>::kRopes;
+  const gemq_latent_decode_t& A = P.a;
+  const int lane = threadIdx.x & 31, blocks = A.rank / 64;
+  int* const err = A.err;
+  Walk<N> walk(P, start);
+  Piece p;
+  int place = 0, freed = 0;  // next latent block of the ring; tiles known to be done
+  uint32_t k = 0, phase = 1;
+  const bool small = A.page_size < kTile;
+  const int per_tile = small ? kTile / A.page_size : 1, quarters = small ? A.page_size / 16 : 4, tiles_a_page = small ? 1 : A.page_size / kTile;
+  const int box_rows = min(A.page_size, kTile), page_bits = A.page_size == 16 ? 4 : 5;  // of small pages
+  const uint32_t ring0 = smem_u32(S.ring[0]), rope0 = smem_u32(S.rope[0]), full0 = smem_u32(&S.full[0]), rope_full0 = smem_u32(&S.rope_full[0]);
+  int rope_at = 0;
+  while (walk.next(p)) {
+    const bool prefix = p.e < A.groups;
+    const int* table = prefix ? A.prefix_table + static_cast<long long>(p.e) * A.prefix_pitch
+                              : A.table + static_cast<long long>(p.e - A.groups) * A.table_pitch;
+    const int pitch = prefix ? A.prefix_pitch : A.table_pitch;
+    int pg = small ? p.t0 * per_tile : tiles_a_page == 1 ? p.t0 : p.t0 / tiles_a_page, row = small ? 0 : (p.t0 - pg * tiles_a_page) * kTile;
+    int base = pg, ids = base + lane < pitch ? table[base + lane] : 0;  // lane i has the id of page base + i
+    for (int i = 0; i < p.n; ++i, ++k) {
+      const int here = small ? (min(p.x.len - (p.t0 + i) * kTile, kTile) + A.page_size - 1) >> page_bits : 1;  // pages of the tile
+      if (pg + here > base + 32) {
+        base = pg;
+        ids = base + lane < pitch ? table[base + lane] : 0;
+      }
+      const bool out = ids < 0 || ids >= A.n_pages;
+      const uint32_t outs = __ballot_sync(0xffffffffu, out) >> (pg - base);
+      int bad = 0;
+      for (int j = 0; j < here; ++j)
+        if ((outs >> j) & 1) bad |= ((1 << quarters) - 1) << (j * quarters);
+      if (lane == 0) {
+        S.bad[k % kSlots] = bad;
+        mbar_arrive(&S.told[k % kSlots]);
+        if (bad) atomicExch(err, GEMQ_LATENT_BAD_PAGE);
+      }
+      const uint32_t bytes = here * box_rows * 128;
+      if (!small) {
+        const int id = __shfl_sync(0xffffffffu, out ? 0 : ids, pg - base);
+        for (int d = 0; d < blocks; d += 2) {
+          wait_for<N != 64>(&S.empty[place >> 1], phase, &S.abort, err);
+          if (elect_lane()) {
+            mbar_expect_at(full0 + place * 4, 2 * kBlock);
+            tma_load_4d_at(ring0 + place * kBlock, &P.latent_map, row, d, id, full0 + place * 4);
+          }
+          __syncwarp();
+          place += 2;
+          if (place == kLatent) { place = 0; phase ^= 1; }
+        }
+        if (static_cast<int>(k) >= kRopes + freed) {
+          wait_for<N != 64>(&S.done[freed % kSlots], (freed / kSlots) & 1, &S.abort, err);
+          ++freed;
+        }
+        if (elect_lane()) {
+          mbar_expect_at(rope_full0 + rope_at * 8, kBlock);
+          tma_load_4d_at(rope0 + rope_at * kBlock, &P.rope_map, row, blocks, id, rope_full0 + rope_at * 8);
+        }
+        __syncwarp();
+      } else {
+        int id[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) id[j] = __shfl_sync(0xffffffffu, out ? 0 : ids, (pg - base + j) & 31);
+        const uint32_t page_bytes = A.page_size * 128;
+        for (int d = 0; d < blocks; d += 2) {
+          wait_for<N != 64>(&S.empty[place >> 1], phase, &S.abort, err);
+          const uint32_t dst = ring0 + place * kBlock, bar = full0 + place * 4;
+          if (elect_lane()) {
+            mbar_expect_at(bar, 2 * bytes);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (j < here) {
+                tma_load_4d_at(dst + j * page_bytes, &P.latent_map, 0, d, id[j], bar);
+                tma_load_4d_at(dst + kBlock + j * page_bytes, &P.latent_map, 0, d + 1, id[j], bar);
+              }
+          }
+          __syncwarp();
+          place += 2;
+          if (place == kLatent) { place = 0; phase ^= 1; }
+        }
+        if (static_cast<int>(k) >= kRopes + freed) {
+          wait_for<N != 64>(&S.done[freed % kSlots], (freed / kSlots) & 1, &S.abort, err);
+          ++freed;
+        }
+        if (elect_lane()) {
+          mbar_expect_at(rope_full0 + rope_at * 8, bytes);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (j < here) tma_load_4d_at(rope0 + rope_at * kBlock + j * page_bytes, &P.rope_map, 0, blocks, id[j], rope_full0 + rope_at * 8);
+        }
+        __syncwarp();
+      }
+      if (++rope_at == kRopes) rope_at = 0;
+      if (small) {
+        pg += per_tile;
+      } else {
+        row += kTile;
+        if (row == A.page_size) { row = 0; ++pg; }
+      }
+    }
+  }
+  // The copies in flight end before the CTA does: the MMAs of the last tile waited for them, unless a wait ran out.
+  if (*reinterpret_cast<volatile int*>(&S.abort))
+    for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+}
+
+// S.  The whole warp runs the loop and one elected lane issues: descriptors stay in uniform registers.
+template <typename T, int N>
+__device__ __forceinline__ void score_tiles(Smem<N>& S, const Args& P, const Start& start, uint32_t tmem) {
+  constexpr int kLatent = Ring<N>::kLatent, kRopes = Ring<N>::kRopes;
+  const gemq_latent_decode_t& A = P.a;
+  const int blocks = A.rank / 64;
+  int* const err = A.err;
+  Walk<N> walk(P, start);
+  Piece p;
+  const uint64_t q0 = umma_desc_k_sw128(smem_u32(S.q[0])), ring0 = umma_desc_k_sw128(smem_u32(S.ring[0])),
+                 rope0 = umma_desc_k_sw128(smem_u32(S.rope[0]));
+  uint32_t k = 0, phase = 0, rope_at = 0, rope_phase = 0;
+  int place = 0;
+  for (uint32_t piece = 0; walk.next(p); ++piece) {
+    const uint32_t idesc = umma_idesc_f16(Pair<T>::kBf16, kTile, p.width());
+    wait_for<N != 64>(&S.q_full, piece & 1, &S.abort, err);
+    for (int i = 0; i < p.n; ++i, ++k) {
+      wait_for<N != 64>(&S.s_free[k & 1], ((k >> 1) & 1) ^ 1, &S.abort, err);
+      const uint32_t s = tmem + (k & 1) * N;
+      for (int d = 0; d < blocks; d += 2) {
+        wait_for<N != 64>(&S.full[place >> 1], phase, &S.abort, err);
+        tc_fence_after_sync();
+        const uint64_t a = ring0 + place * (kBlock >> 4), b = q0 + d * (N * 128 >> 4);
+        if (elect_lane()) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            umma_ss_f16(s, a + (j >> 2) * (kBlock >> 4) + (j & 3) * 2, b + (j >> 2) * (N * 128 >> 4) + (j & 3) * 2, idesc, d != 0 || j != 0);
+        }
+        __syncwarp();
+        place += 2;
+        if (place == kLatent) { place = 0; phase ^= 1; }
+      }
+      wait_for<N != 64>(&S.rope_full[rope_at], rope_phase, &S.abort, err);
+      tc_fence_after_sync();
+      const uint64_t a = rope0 + rope_at * (kBlock >> 4), b = q0 + blocks * (N * 128 >> 4);
+      if (elect_lane()) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) umma_ss_f16(s, a + j * 2, b + j * 2, idesc, 1);
+        umma_commit(&S.s_full[k & 1]);
+        if (i == p.n - 1) umma_commit(&S.q_free);
+      }
+      __syncwarp();
+      if (++rope_at == kRopes) { rope_at = 0; rope_phase ^= 1; }
+    }
+  }
+}
+
+// O.
+template <typename T, int N>
+__device__ __forceinline__ void sum_tiles(Smem<N>& S, const Args& P, const Start& start, uint32_t sums) {
+  constexpr int kLatent = Ring<N>::kLatent, kOs = Smem<N>::kOs;
+  const gemq_latent_decode_t& A = P.a;
+  const int blocks = A.rank / 64;
+  int* const err = A.err;
+  Walk<N> walk(P, start);
+  Piece p;
+  const uint64_t p0 = umma_desc_k_sw128(smem_u32(S.p)), ring0 = umma_desc_mn_sw128(smem_u32(S.ring[0]), kBlock);
+  uint32_t k = 0;
+  int place = 0;
+  for (uint32_t piece = 0; walk.next(p); ++piece) {
+    const uint32_t idesc = umma_idesc_f16(Pair<T>::kBf16, 128, p.width()) | kUmmaTransposeA;
+    const uint32_t acc = sums + piece % kOs * (4 * N);
+    wait_for<N != 64>(&S.o_free[piece % kOs], ((piece / kOs) & 1) ^ 1, &S.abort, err);
+    for (int i = 0; i < p.n; ++i, ++k) {
+      const int steps = cdiv(min(p.x.len - (p.t0 + i) * kTile, kTile), 16);  // of 16 positions
+      wait_for<N != 64>(&S.p_full, k & 1, &S.abort, err);
+      tc_fence_after_sync();
+      // a pair of blocks is free behind its MMAs: S of the tile is complete
+      for (int m = 0; m < blocks / 2; ++m) {
+        const uint64_t a = ring0 + place * (kBlock >> 4);
+        const uint32_t o = acc + m * N;
+        if (elect_lane()) {
+          umma_ss_f16(o, a, p0, idesc, i != 0);
+          if (steps == 4) {
+#pragma unroll
+            for (int s = 1; s < 4; ++s) umma_ss_f16(o, a + s * (2048 >> 4), p0 + s * (32 >> 4), idesc, 1);
+          } else {
+            for (int s = 1; s < steps; ++s) umma_ss_f16(o, a + s * (2048 >> 4), p0 + s * (32 >> 4), idesc, 1);
+          }
+          umma_commit(&S.empty[place >> 1]);
+        }
+        __syncwarp();
+        place = place + 2 == kLatent ? 0 : place + 2;
+      }
+      if (elect_lane()) {
+        umma_commit(&S.done[k % kSlots]);
+        if (i == p.n - 1) umma_commit(&S.o_full[piece % kOs]);
+      }
+      __syncwarp();
+    }
+  }
+}
+
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid_constant__ Args P) {
   constexpr int kLatent = Ring<N>::kLatent, kRopes = Ring<N>::kRopes;
@@ -506,7 +709,6 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
   Smem<N>& S = *reinterpret_cast<Smem<N>*>(smem_raw);
   const gemq_latent_decode_t& A = P.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int blocks = A.rank / 64;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kLatent / 2; ++i) { mbar_init(&S.full[i], 1); mbar_init(&S.empty[i], 1); }
     for (int i = 0; i < kRopes; ++i) mbar_init(&S.rope_full[i], 1);
@@ -522,7 +724,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) tmem_alloc(&S.tmem_base, kTmemCols);
-  if (warp == 0 && lane < 2) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<unsigned long long>(lane ? &P.rope_map : &P.latent_map)) : "memory");
+  if (warp == 0 && lane < 2) prefetch_map(lane ? &P.rope_map : &P.latent_map);
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   // Every CTA adds up the list: a thread has a run of entries.
@@ -584,189 +786,12 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
   __syncthreads();
   const uint32_t tmem = S.tmem_base;
   const Start start = from < to ? S.start : Start{0, 0, 0, 0, 0, 0};
-  int* const err = A.err;
   // 64 rows of queries: 240 registers for the softmax warps; with the others' 88 and 168 below the launch's 3 x 168
   if (warp < kSoftWarp) {
-  if (N == 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-  if (warp == 0) {
-    Walk<N> walk(P, start);
-    Piece p;
-    int place = 0, freed = 0;  // next latent block of the ring; tiles known to be done
-    uint32_t k = 0, phase = 1;
-    const bool small = A.page_size < kTile;
-    const int per_tile = small ? kTile / A.page_size : 1, quarters = small ? A.page_size / 16 : 4, tiles_a_page = small ? 1 : A.page_size / kTile;
-    const int box_rows = min(A.page_size, kTile), page_bits = A.page_size == 16 ? 4 : 5;  // of small pages
-    const uint32_t ring0 = smem_u32(S.ring[0]), rope0 = smem_u32(S.rope[0]), full0 = smem_u32(&S.full[0]), rope_full0 = smem_u32(&S.rope_full[0]);
-    int rope_at = 0;
-    while (walk.next(p)) {
-      const bool prefix = p.e < A.groups;
-      const int* table = prefix ? A.prefix_table + static_cast<long long>(p.e) * A.prefix_pitch
-                                : A.table + static_cast<long long>(p.e - A.groups) * A.table_pitch;
-      const int pitch = prefix ? A.prefix_pitch : A.table_pitch;
-      int pg = small ? p.t0 * per_tile : tiles_a_page == 1 ? p.t0 : p.t0 / tiles_a_page, row = small ? 0 : (p.t0 - pg * tiles_a_page) * kTile;
-      int base = pg, ids = base + lane < pitch ? table[base + lane] : 0;  // lane i has the id of page base + i
-      for (int i = 0; i < p.n; ++i, ++k) {
-        const int here = small ? (min(p.x.len - (p.t0 + i) * kTile, kTile) + A.page_size - 1) >> page_bits : 1;  // pages of the tile
-        if (pg + here > base + 32) {
-          base = pg;
-          ids = base + lane < pitch ? table[base + lane] : 0;
-        }
-        const bool out = ids < 0 || ids >= A.n_pages;
-        const uint32_t outs = __ballot_sync(0xffffffffu, out) >> (pg - base);
-        int bad = 0;
-        for (int j = 0; j < here; ++j)
-          if ((outs >> j) & 1) bad |= ((1 << quarters) - 1) << (j * quarters);
-        if (lane == 0) {
-          S.bad[k % kSlots] = bad;
-          mbar_arrive(&S.told[k % kSlots]);
-          if (bad) atomicExch(err, GEMQ_LATENT_BAD_PAGE);
-        }
-        const uint32_t bytes = here * box_rows * 128;
-        if (!small) {
-          const int id = __shfl_sync(0xffffffffu, out ? 0 : ids, pg - base);
-          for (int d = 0; d < blocks; d += 2) {
-            wait_for<N != 64>(&S.empty[place >> 1], phase, &S.abort, err);
-            if (elect_lane()) {
-              mbar_expect_at(full0 + place * 4, 2 * kBlock);
-              tma_load_4d_at(ring0 + place * kBlock, &P.latent_map, row, d, id, full0 + place * 4);
-            }
-            __syncwarp();
-            place += 2;
-            if (place == kLatent) { place = 0; phase ^= 1; }
-          }
-          if (static_cast<int>(k) >= kRopes + freed) {
-            wait_for<N != 64>(&S.done[freed % kSlots], (freed / kSlots) & 1, &S.abort, err);
-            ++freed;
-          }
-          if (elect_lane()) {
-            mbar_expect_at(rope_full0 + rope_at * 8, kBlock);
-            tma_load_4d_at(rope0 + rope_at * kBlock, &P.rope_map, row, blocks, id, rope_full0 + rope_at * 8);
-          }
-          __syncwarp();
-        } else {
-          int id[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) id[j] = __shfl_sync(0xffffffffu, out ? 0 : ids, (pg - base + j) & 31);
-          const uint32_t page_bytes = A.page_size * 128;
-          for (int d = 0; d < blocks; d += 2) {
-            wait_for<N != 64>(&S.empty[place >> 1], phase, &S.abort, err);
-            const uint32_t dst = ring0 + place * kBlock, bar = full0 + place * 4;
-            if (elect_lane()) {
-              mbar_expect_at(bar, 2 * bytes);
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (j < here) {
-                  tma_load_4d_at(dst + j * page_bytes, &P.latent_map, 0, d, id[j], bar);
-                  tma_load_4d_at(dst + kBlock + j * page_bytes, &P.latent_map, 0, d + 1, id[j], bar);
-                }
-            }
-            __syncwarp();
-            place += 2;
-            if (place == kLatent) { place = 0; phase ^= 1; }
-          }
-          if (static_cast<int>(k) >= kRopes + freed) {
-            wait_for<N != 64>(&S.done[freed % kSlots], (freed / kSlots) & 1, &S.abort, err);
-            ++freed;
-          }
-          if (elect_lane()) {
-            mbar_expect_at(rope_full0 + rope_at * 8, bytes);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (j < here) tma_load_4d_at(rope0 + rope_at * kBlock + j * page_bytes, &P.rope_map, 0, blocks, id[j], rope_full0 + rope_at * 8);
-          }
-          __syncwarp();
-        }
-        if (++rope_at == kRopes) rope_at = 0;
-        if (small) {
-          pg += per_tile;
-        } else {
-          row += kTile;
-          if (row == A.page_size) { row = 0; ++pg; }
-        }
-      }
-    }
-    // The copies in flight end before the CTA does: the MMAs of the last tile waited for them, unless a wait ran out.
-    if (*reinterpret_cast<volatile int*>(&S.abort))
-      for (int i = 0; i < 2000; ++i) __nanosleep(1000);
-  } else if (warp == 1) {
-    // The whole warp runs the loop and one elected lane issues: descriptors stay in uniform registers.
-    Walk<N> walk(P, start);
-    Piece p;
-    const uint64_t q0 = umma_desc_k_sw128(smem_u32(S.q[0])), ring0 = umma_desc_k_sw128(smem_u32(S.ring[0])),
-                   rope0 = umma_desc_k_sw128(smem_u32(S.rope[0]));
-    uint32_t k = 0, phase = 0, rope_at = 0, rope_phase = 0;
-    int place = 0;
-    for (uint32_t piece = 0; walk.next(p); ++piece) {
-      const uint32_t idesc = umma_idesc_f16(Pair<T>::kBf16, kTile, p.width());
-      wait_for<N != 64>(&S.q_full, piece & 1, &S.abort, err);
-      for (int i = 0; i < p.n; ++i, ++k) {
-        wait_for<N != 64>(&S.s_free[k & 1], ((k >> 1) & 1) ^ 1, &S.abort, err);
-        const uint32_t s = tmem + (k & 1) * N;
-        for (int d = 0; d < blocks; d += 2) {
-          wait_for<N != 64>(&S.full[place >> 1], phase, &S.abort, err);
-          tc_fence_after_sync();
-          const uint64_t a = ring0 + place * (kBlock >> 4), b = q0 + d * (N * 128 >> 4);
-          if (elect_lane()) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              umma_ss_f16(s, a + (j >> 2) * (kBlock >> 4) + (j & 3) * 2, b + (j >> 2) * (N * 128 >> 4) + (j & 3) * 2, idesc, d != 0 || j != 0);
-          }
-          __syncwarp();
-          place += 2;
-          if (place == kLatent) { place = 0; phase ^= 1; }
-        }
-        wait_for<N != 64>(&S.rope_full[rope_at], rope_phase, &S.abort, err);
-        tc_fence_after_sync();
-        const uint64_t a = rope0 + rope_at * (kBlock >> 4), b = q0 + blocks * (N * 128 >> 4);
-        if (elect_lane()) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) umma_ss_f16(s, a + j * 2, b + j * 2, idesc, 1);
-          umma_commit(&S.s_full[k & 1]);
-          if (i == p.n - 1) umma_commit(&S.q_free);
-        }
-        __syncwarp();
-        if (++rope_at == kRopes) { rope_at = 0; rope_phase ^= 1; }
-      }
-    }
-  } else if (warp == 2) {
-    Walk<N> walk(P, start);
-    Piece p;
-    const uint64_t p0 = umma_desc_k_sw128(smem_u32(S.p)), ring0 = umma_desc_mn_sw128(smem_u32(S.ring[0]), kBlock);
-    uint32_t k = 0;
-    int place = 0;
-    for (uint32_t piece = 0; walk.next(p); ++piece) {
-      const uint32_t idesc = umma_idesc_f16(Pair<T>::kBf16, 128, p.width()) | kUmmaTransposeA;
-      const uint32_t acc = tmem + kTmemO + piece % kOs * (4 * N);
-      wait_for<N != 64>(&S.o_free[piece % kOs], ((piece / kOs) & 1) ^ 1, &S.abort, err);
-      for (int i = 0; i < p.n; ++i, ++k) {
-        const int steps = cdiv(min(p.x.len - (p.t0 + i) * kTile, kTile), 16);  // of 16 positions
-        wait_for<N != 64>(&S.p_full, k & 1, &S.abort, err);
-        tc_fence_after_sync();
-        // a pair of blocks is free behind its MMAs: S of the tile is complete
-        for (int m = 0; m < blocks / 2; ++m) {
-          const uint64_t a = ring0 + place * (kBlock >> 4);
-          const uint32_t o = acc + m * N;
-          if (elect_lane()) {
-            umma_ss_f16(o, a, p0, idesc, i != 0);
-            if (steps == 4) {
-#pragma unroll
-              for (int s = 1; s < 4; ++s) umma_ss_f16(o, a + s * (2048 >> 4), p0 + s * (32 >> 4), idesc, 1);
-            } else {
-              for (int s = 1; s < steps; ++s) umma_ss_f16(o, a + s * (2048 >> 4), p0 + s * (32 >> 4), idesc, 1);
-            }
-            umma_commit(&S.empty[place >> 1]);
-          }
-          __syncwarp();
-          place = place + 2 == kLatent ? 0 : place + 2;
-        }
-        if (elect_lane()) {
-          umma_commit(&S.done[k % kSlots]);
-          if (i == p.n - 1) umma_commit(&S.o_full[piece % kOs]);
-        }
-        __syncwarp();
-      }
-    }
-  }
+    if (N == 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == 0) load_tiles<N>(S, P, start);
+    else if (warp == 1) score_tiles<T, N>(S, P, start, tmem);
+    else if (warp == 2) sum_tiles<T, N>(S, P, start, tmem + kTmemO);
   } else if (warp >= kEdgeWarp) {
     Walk<N> ahead(P, start), walk(P, start);
     Piece q, p;

@@ -135,6 +135,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __gri
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) tmem_alloc(&S.tmem_base, 512);
+  if (warp == 2 && lane < 4) prefetch_map(lane == 0 ? &P.q_nope : lane == 1 ? &P.q_rope : lane == 2 ? &P.kv : &P.k_rope);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (warp == 0) {
     // The block's sequence: 32 sequences at a time.  Behind the last there is one more, of the query rows that no sequence has.

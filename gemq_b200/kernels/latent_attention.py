@@ -104,7 +104,8 @@ def latent_append(kv: Tensor, q_rope: Tensor, norm_weight: Tensor, eps: float, i
     rank, page_stride = _check_cache(cache, kv.dtype)
     require(kv.dim() == 2 and kv.shape[1] == rank + ROPE, f"kv must be [tokens, {rank + ROPE}]")
     T = kv.shape[0]
-    require(q_rope.dim() == 3 and q_rope.shape[0] == T and q_rope.shape[2] == ROPE and q_rope.dtype == kv.dtype, "q_rope must be [tokens, heads, 64] of kv's type")
+    require(q_rope.dim() == 3 and q_rope.shape[0] == T and q_rope.shape[2] == ROPE and q_rope.dtype == kv.dtype,
+            "q_rope must be [tokens, heads, 64] of kv's type")
     require(tuple(norm_weight.shape) == (rank,) and norm_weight.dtype == kv.dtype, "norm_weight must be [rank] of kv's type")
     _ints("inv_freq", inv_freq, torch.float32, (ROPE // 2,))
     _ints("positions", positions, torch.int64, (T,))
@@ -119,9 +120,9 @@ def latent_append(kv: Tensor, q_rope: Tensor, norm_weight: Tensor, eps: float, i
     q_strides = _strides("q_rope", q_rope) if H else (0, 0)
     with _on(dev):
         _capi.check("gemq_latent_append", _capi.lib.gemq_latent_append(
-            kv.data_ptr(), kv_stride, q_rope.data_ptr() if H else None, *q_strides, norm_weight.data_ptr(), eps, inv_freq.data_ptr(), rope_scale, positions.data_ptr(), slots.data_ptr(), cache.data_ptr(),
-            page_stride, cache.shape[0], cache.shape[1], rows.data_ptr(), q_out.data_ptr() if H else None, T, H, rank,
-            int(kv.dtype == torch.bfloat16), error_word(dev).data_ptr(), stream_ptr(dev)))
+            kv.data_ptr(), kv_stride, q_rope.data_ptr() if H else None, *q_strides, norm_weight.data_ptr(), eps, inv_freq.data_ptr(),
+            rope_scale, positions.data_ptr(), slots.data_ptr(), cache.data_ptr(), page_stride, cache.shape[0], cache.shape[1], rows.data_ptr(),
+            q_out.data_ptr() if H else None, T, H, rank, int(kv.dtype == torch.bfloat16), error_word(dev).data_ptr(), stream_ptr(dev)))
     return q_out, rows
 
 
