@@ -3,7 +3,8 @@
 //
 //   row = { c * rsqrt(mean(c^2) + eps) * w,  rot(k, p) },   rot(x, p)[2i, 2i+1] = m * (x0 cos a - x1 sin a, x0 sin a + x1 cos a),  a = p * f_i
 //
-// Both move bytes and compute next to nothing.
+// Both move bytes and compute next to nothing.  Measured: 8191 rows of rank 512 with 16 heads' queries, 62 MB: 12.4 us (5.0 TB/s; 15.4 before
+// the queries were asked for ahead of the norm); 391 pages in 27 layers, 1.56 GB: 269 us (5.8 TB/s, 0.88 of a plain copy's rate).
 #include "latent.cuh"
 
 namespace gemq {

@@ -22,6 +22,12 @@
 // The maximum that the weights refer to moves only when a row's scores exceed it by 2^8: O is corrected in tensor memory a few times per
 // sequence.  Rows behind what is seen are zeroed in shared memory before they are multiplied by weights of 0: what lies there may be NaN.
 // Every wait is bounded.
+//
+// Measured (rank 512; the call with both launches): 37 sequences of 60 to 9000 positions, 16 heads, 80 MB: 33 us, 2.4 TB/s; 2 sequences of 70,001
+// and 131,072, 48 rows each, 232 MB: 65 us, 3.6 TB/s; 64 sequences behind a prefix of 8000, 18 GFLOP: 48 us; one of 700: 11 us.  A CTA's 64
+// positions take 3100 to 3300 cycles with all SMs at work: 16 rows what HBM gives (3100), 64 rows the two products' reads of shared memory
+// (2000 cycles of MMAs, 340 KB at 128 bytes a cycle) and a ring of two tiles.  The rest is fixed: 3 to 5 us to the first copy, 3 to the first
+// weights, 1 to 4 for results (64 rows: 131 KB at 32 bytes a cycle), 2 to 6 for the join.
 #include "latent.cuh"
 
 namespace gemq {

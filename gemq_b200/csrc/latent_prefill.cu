@@ -18,6 +18,10 @@
 // What a query must not see is given a weight of 0.  If such a row of v holds an infinity or a NaN the product still is NaN: a block with a
 // result that is not finite is computed once more, and warp 3 sets to zero, in the tiles that not all of its queries see whole, what
 // is hidden from all and what is not finite; a query that sees one of the latter gets a NaN for its weight.  Every wait is bounded.
+//
+// Measured: 8192 queries x 16 heads, 344 GFLOP: 336 us in a loop of calls (1.02 PFLOP/s at 1.7 GHz, the power limit), 284 in short bursts
+// (1.21); a round of both tiles 3550 to 3900 cycles of 2560 of MMAs.  Tried: values in a ring of their own depth with the keys (the tiles fall into
+// step and share the exponentials' units: 5100 to 5500 cycles; made to take turns: 3700 and the same time).
 #include "latent.cuh"
 
 namespace gemq {
