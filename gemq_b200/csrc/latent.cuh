@@ -38,8 +38,7 @@ __device__ __forceinline__ int clamp_length(int n, int pitch, int page_size, int
   return n < 0 ? 0 : static_cast<int>(most);
 }
 
-// Entry i of n + 1 offsets that are meant to rise from 0 to at most `most`: where they do not, as if they did (every entry the largest
-// up to it, within 0 .. most).  By one thread, for checks; kernels scan.
+// Whether n + 1 offsets rise from 0 to at most `most` (or to it).  By one thread of the launch, to report; each use is clamped by itself.
 __device__ __forceinline__ bool offsets_ok(const int* v, int n, int most, bool to_the_end) {
   int last = 0;
   bool ok = v[0] == 0;

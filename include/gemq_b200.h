@@ -322,7 +322,8 @@ int gemq_step_attention(const void* qkv, const float* inv_freq, const int64_t* p
  * when the device data is out of range (GEMQ_LATENT_*); such entries are never used as an index.  */
 enum {
   GEMQ_LATENT_BAD_PAGE = 41,   /* page id outside the cache: what would see the page is NaN, a copy is skipped */
-  GEMQ_LATENT_BAD_LENGTH = 42, /* negative length, or one beyond its page table: clamped; offsets that do not rise: as if they did */
+  GEMQ_LATENT_BAD_LENGTH = 42, /* negative length, or one beyond its page table: clamped; offsets that do not rise from 0 within their tensor:
+                                  what they ask for is undefined, nothing outside the tensors is touched */
   GEMQ_LATENT_BAD_SLOT = 43,   /* slot outside the cache: the row is not stored (-1 is not an error) */
   GEMQ_LATENT_WAIT = 44        /* a wait inside a kernel ran out */
 };

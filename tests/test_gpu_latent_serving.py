@@ -29,7 +29,7 @@ def make_layer(dtype, seed, quantised):
 
 def weight(linear):
     from gemq_b200.inference.latent_attention import _weight
-    return _weight(linear, torch.float64)
+    return _weight(linear, torch.float64).detach()
 
 
 def reference(layer, hidden):
@@ -103,6 +103,35 @@ def test_a_run_of_all_of_them(dtype, quantised):
     s.step([d, b, e], [1] * 3, s.cache.plan_decode([d, b, e]))
     s.step([d, e, b], [1] * 3, s.cache.plan_decode([d, e, b], groups=[2, 1]))
     assert latent_error() == 0
+
+
+@pytest.mark.parametrize("q_rank", [None, 96])
+def test_layer_from_hugging_face(q_rank):
+    """The layer made of a Hugging Face module against that module, in 32 bits, over one sequence: a prompt, then tokens one by one."""
+    M = pytest.importorskip("transformers.models.deepseek_v2.modeling_deepseek_v2")
+    from transformers import DeepseekV2Config
+    from gemq_b200.inference import LatentAttention, PagedLatentCache
+    cfg = DeepseekV2Config(hidden_size=D, num_attention_heads=H, num_key_value_heads=H, kv_lora_rank=RANK, q_lora_rank=q_rank,
+                           qk_nope_head_dim=NOPE, qk_rope_head_dim=ROPE, v_head_dim=VALUE, num_hidden_layers=1, vocab_size=64, intermediate_size=64)
+    cfg._attn_implementation = "eager"
+    torch.manual_seed(5)
+    hf = M.DeepseekV2Attention(cfg, 0).cuda()
+    for p in hf.parameters():
+        p.data = (p.data + torch.randn_like(p) * (0.1 if p.dim() == 1 else p.shape[1] ** -0.5)).half().float()
+    x = torch.randn(1, 50, D, device="cuda").half().float()
+    pos = torch.arange(50, device="cuda")[None]
+    mask = torch.full((50, 50), float("-inf"), device="cuda").triu(1)[None, None]
+    with torch.no_grad():
+        want = hf(x, mask, position_embeddings=M.DeepseekV2RotaryEmbedding(cfg).cuda()(x, pos))[0][0]
+    layer = LatentAttention.from_hf(cfg, hf.half())
+    cache = PagedLatentCache(1, 4, 16, RANK, torch.float16)
+    seq = cache.new()
+    got = [layer(x[0, :41].half(), cache, 0, cache.plan_prefill([seq], [41]))]
+    for i in range(41, 50):
+        got.append(layer(x[0, i:i + 1].half(), cache, 0, cache.plan_decode([seq])))
+    got = torch.cat(got).float()
+    # the roundings of a run's step, and two more where the queries come through a norm
+    assert float((got - want).norm() / want.norm()) < (6 + 5 * (1 + 2 * 3)) * torch.finfo(torch.float16).eps / 2
 
 
 def test_a_decode_step_captured_and_replayed():

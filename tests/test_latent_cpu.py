@@ -268,9 +268,27 @@ def test_attention_layer_refuses():
     lin = lambda o, i: torch.nn.Linear(i, o, bias=False)  # noqa: E731
     with pytest.raises(ValueError, match="kv_b_proj"):
         LatentAttention(lin(768, 32), lin(192, 32), torch.ones(128), 1e-6, lin(1000, 128), lin(32, 512), 4, torch.ones(32))
+    with pytest.raises(ValueError, match="bias"):
+        LatentAttention(lin(768, 32), lin(192, 32), torch.ones(128), 1e-6, torch.nn.Linear(128, 1024), lin(32, 512), 4, torch.ones(32))
+    with pytest.raises(ValueError, match="inv_freq"):
+        LatentAttention(lin(768, 32), lin(192, 32), torch.ones(128), 1e-6, lin(1024, 128), lin(32, 512), 4, torch.ones(64))
     cfg = SimpleNamespace(qk_nope_head_dim=128, qk_rope_head_dim=64, v_head_dim=128, rope_scaling={"type": "yarn"}, num_attention_heads=4)
-    with pytest.raises(ValueError, match="rope_scaling"):
+    with pytest.raises(ValueError, match="rotation"):
         LatentAttention.from_hf(cfg, None)
     cfg.v_head_dim = 64
     with pytest.raises(ValueError, match="128"):
         LatentAttention.from_hf(cfg, None)
+
+
+def test_attention_layer_follows_its_weights():
+    """The halves that the absorbed form reads are those of the weight that was loaded; the frequencies stay in 32 bits."""
+    from gemq_b200.inference import LatentAttention
+    make = lambda: LatentAttention(*(torch.nn.Linear(i, o, bias=False) for i, o in ((32, 768), (32, 192))), torch.rand(128), 1e-6,  # noqa: E731
+                                   torch.nn.Linear(128, 1024, bias=False), torch.nn.Linear(512, 32, bias=False), 4, torch.rand(32))
+    a, b = make(), make()
+    assert not torch.equal(a.w_keys, b.w_keys) and not any(k.startswith("w_") for k in a.state_dict())
+    a.load_state_dict(b.state_dict())
+    w = b.kv_b_proj.weight.view(4, 256, 128)
+    assert torch.equal(a.w_keys, w[:, :128]) and torch.equal(a.w_values, w[:, 128:].transpose(1, 2)) and torch.equal(a.norm_weight, b.norm_weight)
+    a.half()
+    assert a.w_keys.dtype == a.norm_weight.dtype == f16 and a.inv_freq.dtype == torch.float32
