@@ -299,9 +299,10 @@ __device__ __forceinline__ void softmax_piece(Smem<N>& S, const Args& P, const P
         float top = -INFINITY;
 #pragma unroll 4
         for (int r = 0; r < 32; ++r) top = fmaxf(top, scratch[r * NP + me]);
-        // relative to the reference so far; a row that has none takes what there is
-        const float up = my_none ? top - kOffset : fmaxf(top - kOffset, 0.f);
-        const bool nothing = up == -INFINITY;
+        // Relative to the reference so far; a row that has none takes what there is.  Only a row of its own scores: which others stand beside it
+        // in the tile, and what those see, is to change none of its bits.
+        const float up = my_none || top > kOffset + 8.f ? top - kOffset : 0.f;
+        const bool nothing = my_none && up == -INFINITY;
         const float by = nothing ? 0.f : up;
         still = nothing && S.limit[me] > 0;
         S.wmax[0][me] = by;

@@ -367,7 +367,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __gri
         for (int c = 4; c + 1 < kRows; c += 2) most4[(c >> 1) & 3] = max3(most4[(c >> 1) & 3], v[c], v[c + 1]);
         const float top = fmaxf(fmaxf(most4[0], most4[1]), fmaxf(most4[2], most4[3]));
         if (__any_sync(0xffffffffu, none ? top > -INFINITY : top > kOffset + 8.f)) {
-          const float up = none ? top - kOffset : fmaxf(top - kOffset, 0.f), by = up == -INFINITY ? 0.f : up;
+          // a row's own scores decide: its neighbours in the warp, and what those see, are to change none of its bits
+          const float up = none || top > kOffset + 8.f ? top - kOffset : 0.f, by = up == -INFINITY ? 0.f : up;
           const float f = none ? 1.f : exp2_fast(-by);
           none = none && up == -INFINITY;
           ref += by;

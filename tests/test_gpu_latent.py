@@ -521,3 +521,65 @@ def test_copy_pages(layers, pages, page, width, dtype):
         copy_pages(cache, torch.tensor([0, bad], device="cuda"), torch.tensor([bad, 1], device="cuda"))
         assert latent_error() == 41 and torch.equal(big, want)
     copy_pages(cache, src[:0], dst[:0])
+
+
+# ---- what others in the same tile hold ------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_large_numbers_of_others_change_no_bit_of_decode(dtype):
+    """Pieces of several tiles, so that the reference of a row's weights may move behind the first: a large finite row that only the later queries see,
+    and a large query of one head, leave every other query bit for bit what it was."""
+    from gemq_b200.kernels import latent_decode
+    lens = [400 + 7 * i % 200 for i in range(300)]
+    q_latent, q_rope, cache, table, n, rows = decode_case(lens, 4, 16, 512, 64, dtype, seed=1)
+    want = latent_decode(q_latent, q_rope, cache, table, n, 192 ** -0.5)
+    bad = cache.clone()
+    for b, (pages, length) in enumerate(rows):  # seen by queries 2 and 3
+        bad[pages[(length - 2) // 64], (length - 2) % 64] = 60 * torch.cat([q_latent[b, 3, 5], q_rope[b, 3, 5]])
+    assert bool(bad[rows[0][0][0]].isfinite().all())
+    got = latent_decode(q_latent, q_rope, bad, table, n, 192 ** -0.5)
+    assert not torch.equal(got[0][:, 2:], want[0][:, 2:])
+    assert all(torch.equal(a[:, :2], b[:, :2]) for a, b in zip(got, want))
+    large = q_latent.clone()
+    large[:, :, 5] *= 64
+    got = latent_decode(large, q_rope, cache, table, n, 192 ** -0.5)
+    others = [h for h in range(16) if h != 5]
+    assert all(torch.equal(a[:, :, others], b[:, :, others]) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_large_queries_of_others_change_no_bit_behind_a_prefix(dtype):
+    """Rows of several sequences stand in one tile of queries: a large one is its own sequence's."""
+    from gemq_b200.kernels import latent_decode_shared
+    B = 40
+    q_latent, q_rope, cache, table, n, _ = decode_case([30] * B + [40000], 1, 16, 512, 64, dtype, seed=2)
+    args = (q_rope[:B], cache, table[:B].contiguous(), n[:B].contiguous(), table[B:].contiguous(), n[B:].contiguous(),
+            torch.tensor([0, B], dtype=torch.int32, device="cuda"), 192 ** -0.5)
+    want = latent_decode_shared(q_latent[:B], *args)
+    large = q_latent[:B].clone()
+    large[::4] *= 64
+    got = latent_decode_shared(large, *args)
+    keep = [b for b in range(B) if b % 4]
+    assert all(torch.equal(a[keep], b[keep]) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("at", [140, 200, 270])
+def test_large_numbers_of_others_change_no_bit_of_prefill(at, dtype):
+    """A large finite key in a tile behind the first, and a large query, beside queries of the same warp."""
+    from gemq_b200.kernels import latent_prefill
+    q, kv, k_rope, cu_q, cu_k = prefill_case([(300, 300), (40, 340)], 16, dtype)
+    args = lambda q, kv: (q[..., :NOPE], q[..., NOPE:], kv, k_rope, cu_q, cu_k, 192 ** -0.5)  # noqa: E731
+    want = latent_prefill(*args(q, kv))
+    bad = kv.clone()
+    bad[at, :, :NOPE] = 60 * q[at + 10, :, :NOPE]  # aligned with a later query of the tile
+    assert bool(bad.isfinite().all())
+    got = latent_prefill(*args(q, bad))
+    assert not torch.equal(got[0][at:300], want[0][at:300])
+    keep = list(range(at)) + list(range(300, 340))
+    assert all(torch.equal(a[keep], b[keep]) for a, b in zip(got, want))
+    large = q.clone()
+    large[at] *= 64
+    large[320] *= 64
+    got = latent_prefill(*args(large, kv))
+    keep = [i for i in range(340) if i not in (at, 320)]
+    assert all(torch.equal(a[keep], b[keep]) for a, b in zip(got, want))
