@@ -38,15 +38,15 @@ __device__ __forceinline__ int clamp_length(int n, int pitch, int page_size, int
   return n < 0 ? 0 : static_cast<int>(most);
 }
 
-// Whether n + 1 offsets rise from 0 to at most `most` (or to it).  By one thread of the launch, to report; each use is clamped by itself.
-__device__ __forceinline__ bool offsets_ok(const int* v, int n, int most, bool to_the_end) {
+// Whether n + 1 offsets rise from 0 to at most `most`.  By one thread of the launch, to report; each use is clamped by itself.
+__device__ __forceinline__ bool offsets_ok(const int* v, int n, int most) {
   int last = 0;
   bool ok = v[0] == 0;
   for (int i = 1; i <= n; ++i) {
     ok = ok && v[i] >= last && v[i] <= most;
     last = v[i];
   }
-  return ok && (!to_the_end || last == most);
+  return ok;
 }
 
 // A wait that runs out (about a second) is reported and ends all waits of the CTA.

@@ -81,7 +81,7 @@ struct Smem {
 struct Args {
   CUtensorMap latent_map, rope_map;
   gemq_latent_decode_t a;
-  int* ctl;          // [0] cost of the list, then per entry: where it begins in it, first row tile
+  int* ctl;          // [0] cost of the list, -1 without one (start_wrong); from [2] per entry: where it begins in it, first row tile
   float* part_o;     // [slots][N][rank]
   float2* part_ml;   // [slots][N]: reference of the weights (in powers of two) and their sum
   int slots;
@@ -116,6 +116,13 @@ __device__ __forceinline__ Entry entry_here(const Args& P, int e) {
 }
 // Out of line, as it is wanted in many places: see wait_on.
 __device__ __noinline__ Entry entry_of(const Args& P, int e) { return entry_here(P, e); }
+
+// Starts rise from 0 to the batch: this is what group g says of it.  Where they do not there is no list, and results are NaN: groups that each
+// had the batch would make one beyond its 32 bits, and more pieces than there are slots.
+__device__ __forceinline__ bool start_wrong(const gemq_latent_decode_t& A, int g) {
+  const int from = A.starts[g], to = A.starts[g + 1];
+  return from > to || (g == 0 && from != 0) || (g == A.groups - 1 && to != A.batch);
+}
 
 // Tile t of a row tile that begins at `base` of the list is at base + piece + 4 t.  The list is cut into shares of `share` or, the first
 // `longer` of them, one more.  A share is a tile or more: no CTA between a row tile's first and last is without one.
@@ -456,9 +463,10 @@ __device__ __forceinline__ void finish_piece(Smem<N>& S, const Args& P, const Pi
   const uint32_t lanes = static_cast<uint32_t>(32 * quad) << 16;
   const bool prefix = p.e < A.groups, whole = p.whole() && A.groups == 0;
   const int slot = slot_of(A.groups > 0, p.rt, blockIdx.x, p.last());
-  if (slot >= P.slots) atomicExch(A.err, GEMQ_LATENT_BAD_LENGTH);
+  const bool fits = static_cast<unsigned>(slot) < static_cast<unsigned>(P.slots);
+  if (!fits) atomicExch(A.err, GEMQ_LATENT_BAD_LENGTH);
   wait_for<N != 64>(&S.r_full, piece & 1, &S.abort, A.err);
-  if (me < p.rows && (whole || slot < P.slots)) {
+  if (me < p.rows && (whole || fits)) {
     const float2 r = S.result[me];
     if (whole) {
       const bool empty = limit_of(P, p.x, prefix, p.row0 + me) <= 0;
@@ -495,7 +503,7 @@ __device__ __forceinline__ void finish_piece(Smem<N>& S, const Args& P, const Pi
           }
         out += 2 * A.rank;
       }
-    } else if (slot < P.slots) {
+    } else if (fits) {
       float* out = P.part_o + (static_cast<long long>(slot) * N + j) * A.rank + me;
 #pragma unroll
       for (int x = 0; x < 16; ++x, out += A.rank)
@@ -748,15 +756,15 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
   // entries a lane: no gain).
   const int entries = A.groups + A.batch, c = blockIdx.x;
   Start start = {0, 0, 0, 0, 0, 0, {0, 0, 0, 0, 0, 0}};
-  auto share = [&](int total) {
-    const Cut cut(total, gridDim.x);
+  auto share = [&](int total, bool wrong) {
+    const Cut cut(wrong ? 0 : total, gridDim.x);
     if (c < cut.ctas) {
       start.from = cut.from(c);
       start.to = cut.from(c + 1);
     }
     if (c == 0 && threadIdx.x == 0) {
-      P.ctl[0] = total;
-      if (A.groups > 0 && !offsets_ok(A.starts, A.groups, A.batch, true)) atomicExch(A.err, GEMQ_LATENT_BAD_LENGTH);
+      P.ctl[0] = wrong ? -1 : total;
+      if (wrong) atomicExch(A.err, GEMQ_LATENT_BAD_LENGTH);
     }
   };
   constexpr int kFew = 32;
@@ -770,7 +778,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
       const int a = __shfl_up_sync(0xffffffffu, upto, d), b = __shfl_up_sync(0xffffffffu, rts, d);
       if (lane >= d) { upto += a; rts += b; }
     }
-    share(__shfl_sync(0xffffffffu, upto, 31));
+    share(__shfl_sync(0xffffffffu, upto, 31), A.groups > 0 && __any_sync(0xffffffffu, lane < A.groups && start_wrong(A, lane)));
     const int begin = upto - n * x.cost;
     rts -= n;
     if (c == 0 && warp == 0 && lane < entries) {
@@ -791,11 +799,13 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     }
   }
   int cost = 0, rts = 0, before = 0, rts_before = 0;
+  bool wrong = false;
   const int run = cdiv(entries, kThreads);
   if (entries > kFew) {
     for (int k = 0; k < run; ++k) {
       const int e = static_cast<int>(threadIdx.x) * run + k;
       if (e >= entries) break;
+      if (e < A.groups) wrong = wrong || start_wrong(A, e);
       const Entry x = entry_of(P, e);
       const int n = cdiv(x.rows, N);
       cost += n * x.cost;
@@ -811,7 +821,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     if (lane == 31) { S.sums[warp][0] = before; S.sums[warp][1] = rts_before; }
   }
   tc_fence_before_sync();
-  __syncthreads();
+  if (entries <= kFew || A.groups == 0) __syncthreads();
+  else wrong = __syncthreads_or(wrong);
   tc_fence_after_sync();
   // Only now: a CTA of the next kernel must not take this SM's tensor memory first.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -824,7 +835,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
       if (w < warp) { before += S.sums[w][0]; rts_before += S.sums[w][1]; }
       total += S.sums[w][0];
     }
-    share(total);
+    share(total, wrong);
     if (c == 0 || (start.from >= before && start.from < before + cost)) {
       int at = before, rto = rts_before;
       for (int k = 0; k < run; ++k) {
@@ -900,8 +911,10 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 1 ? 6 : 2) latent_
   // Ahead of every read, those of the inputs too: what kernels before have written is visible behind a wait of the reader.  (Lengths and starts
   // read ahead of it: 0.3 us less, 0.6 with prefixes.)
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int total = P.ctl[0];
+  const bool sound = total >= 0;
   const int per_row = W == 1 ? 1 : cuts, bits = 31 - __clz(N);
-  const Find cut(P.ctl[0], sms);
+  const Find cut(total, sms);
   for (int job = blockIdx.x; job < A.batch * A.steps * A.heads * per_row; job += gridDim.x) {
     const int row = W == 1 ? job : cuts == 4 ? job >> 2 : job / cuts, at4 = (W == 1 ? warp : job - row * cuts) * 32 + lane;
     const Row q(P, row);
@@ -926,7 +939,7 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 1 ? 6 : 2) latent_
     int rt[2] = {0, 0}, first[2] = {0, 0}, count[2] = {0, 0}, at[2] = {0, 0};  // runs of pieces: of the group's prefix, of the sequence's own tiles
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      if (x[k].tiles > 0) {
+      if (x[k].tiles > 0 && sound) {
         const int2 list = k ? own : *reinterpret_cast<const int2*>(P.ctl + 2 + 2 * g);
         const int r = row - x[k].row0, base = list.x + (r >> bits) * x[k].cost;
         const int c0 = cut.cta_of(base + x[k].piece), c1 = cut.cta_of(base + x[k].piece + 4 * (x[k].tiles - 1));
@@ -939,7 +952,7 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 1 ? 6 : 2) latent_
     if (A.groups == 0 && count[1] == 1) continue;  // written already
     const int pieces = count[0] + count[1];
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    float l = 0.f, top = -INFINITY;
+    float l = sound ? 0.f : __int_as_float(0x7fc00000), top = -INFINITY;
     if (W == 1 && warp >= cuts) continue;
     for (int i0 = W == 1 ? 0 : warp; i0 < pieces; i0 += W * kJoinAhead) {
       float4 v[kJoinAhead];
@@ -951,7 +964,7 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 1 ? 6 : 2) latent_
                                    : slot_of(A.groups > 0, rt[1], first[1] + i - count[0], i == pieces - 1);
         ml[k] = make_float2(-INFINITY, 0.f);
         v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (i < pieces && s < P.slots) {
+        if (i < pieces && static_cast<unsigned>(s) < static_cast<unsigned>(P.slots)) {
           const long long from = static_cast<long long>(s) * N + (i < count[0] ? at[0] : at[1]);
           ml[k] = P.part_ml[from];
           v[k] = reinterpret_cast<const float4*>(P.part_o + from * A.rank)[at4];
@@ -997,7 +1010,7 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 1 ? 6 : 2) latent_
       }
     }
     if (W == 1 || warp == 0) {
-      const bool empty = len - hidden <= 0;
+      const bool empty = len - hidden <= 0 && sound;
       const float f = 1.f / l;
       reinterpret_cast<uint2*>(static_cast<T*>(A.out) + static_cast<long long>(row) * A.rank)[at4] =
           empty ? make_uint2(0, 0) : make_uint2(Pair<T>::r(o.x * f, o.y * f), Pair<T>::r(o.z * f, o.w * f));

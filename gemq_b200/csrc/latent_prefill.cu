@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __gri
     }
     if (!__any_sync(0xffffffffu, hit) && lane == 0) S.item = {0, 0, 0, 0, 0};
   }
-  if (blockIdx.x == 0 && threadIdx.x == 32 * 11 && !(offsets_ok(A.cu_q, A.batch, A.q_rows, false) && offsets_ok(A.cu_k, A.batch, A.k_rows, false)))
+  if (blockIdx.x == 0 && threadIdx.x == 32 * 11 && !(offsets_ok(A.cu_q, A.batch, A.q_rows) && offsets_ok(A.cu_k, A.batch, A.k_rows)))
     atomicExch(err, GEMQ_LATENT_BAD_LENGTH);
   tc_fence_before_sync();
   __syncthreads();

@@ -194,7 +194,7 @@ def latent_decode_shared(q_latent: Tensor, q_rope: Tensor, cache: Tensor, table:
     """``latent_decode`` for a batch in which sequences ``starts[g] .. starts[g + 1] - 1`` begin with the same ``prefix_lens[g]``
     rows, the pages ``prefix_table[g]``; ``table`` and ``lens`` hold what each sequence has behind them.  The result is that of
     the joined sequences; a prefix is read and multiplied once for all its sequences.  ``starts [groups + 1]`` rises
-    from 0 to the batch."""
+    from 0 to the batch; where it does not, that is reported and all results are NaN."""
     return _decode(q_latent, q_rope, cache, table, lens, scale, prefix_table, prefix_lens, starts)
 
 

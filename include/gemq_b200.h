@@ -323,7 +323,8 @@ int gemq_step_attention(const void* qkv, const float* inv_freq, const int64_t* p
 enum {
   GEMQ_LATENT_BAD_PAGE = 41,   /* page id outside the cache: what would see the page is NaN, a copy is skipped */
   GEMQ_LATENT_BAD_LENGTH = 42, /* negative length, or one beyond its page table: clamped; offsets that do not rise from 0 within their tensor:
-                                  what they ask for is undefined, nothing outside the tensors is touched */
+                                  what they ask for is undefined, nothing outside the tensors is touched; with such `starts` all results
+                                  are NaN */
   GEMQ_LATENT_BAD_SLOT = 43,   /* slot outside the cache: the row is not stored (-1 is not an error) */
   GEMQ_LATENT_WAIT = 44        /* a wait inside a kernel ran out */
 };

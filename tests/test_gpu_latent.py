@@ -583,3 +583,21 @@ def test_large_numbers_of_others_change_no_bit_of_prefill(at, dtype):
     got = latent_prefill(*args(large, kv))
     keep = [i for i in range(340) if i not in (at, 320)]
     assert all(torch.equal(a[keep], b[keep]) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("B,G,pitch", [(4, 6, 3), (40, 7, 40), (512, 600, 20000)])
+def test_decode_shared_of_starts_that_go_back(B, G, pitch):
+    """Starts by which every other group has the whole batch: reported, and all results are NaN.  (The last of them asks for more than 2^31 quarters
+    of a tile.)"""
+    from gemq_b200.kernels import latent_decode_shared, latent_error
+    q_latent, q_rope, cache, table, n, _ = decode_case([1 + 9 * i % 80 for i in range(B)], 1, 16, 512, 64, torch.bfloat16)
+    prefix = torch.zeros(G, pitch, dtype=torch.int32, device="cuda")
+    full, none = torch.full((G,), 64 * pitch, dtype=torch.int32, device="cuda"), torch.zeros(G, dtype=torch.int32, device="cuda")
+    run = lambda lens, starts: latent_decode_shared(q_latent, q_rope, cache, table, n, prefix, lens,  # noqa: E731
+                                                    torch.tensor(starts, dtype=torch.int32, device="cuda"), 0.07)
+    run(none, [0] + [B] * G)
+    assert latent_error() == 0
+    for starts in ([B * (g % 2) for g in range(G)] + [B], [0] + [B + 1] * G, [-1] + [B] * G, [0] * (G + 1), [B] * (G + 1), [0] + [2 ** 31 - 1, -2 ** 31] * (G // 2) + [B] * (G % 2)):
+        got = run(full, starts)
+        assert latent_error() == 42
+        assert all(bool(t.isnan().all()) for t in got), starts
