@@ -147,7 +147,8 @@ def _decode(q_latent, q_rope, cache, table, lens, scale, prefix_table=None, pref
         _ints("prefix_table", prefix_table, torch.int32, (G, prefix_table.shape[1]))
         _ints("prefix_lens", prefix_lens, torch.int32, (G,))
         _ints("starts", starts, torch.int32, (G + 1,))
-        A.prefix_table, A.prefix_pitch, A.prefix_lens = prefix_table.data_ptr(), prefix_table.shape[1], prefix_lens.data_ptr()
+        A.prefix_table, A.prefix_pitch = prefix_table.data_ptr() or cache.data_ptr(), prefix_table.shape[1]
+        A.prefix_lens = prefix_lens.data_ptr()
         A.starts, A.groups = starts.data_ptr(), G
     if B == 0:
         return out, lse

@@ -601,3 +601,14 @@ def test_decode_shared_of_starts_that_go_back(B, G, pitch):
         got = run(full, starts)
         assert latent_error() == 42
         assert all(bool(t.isnan().all()) for t in got), starts
+
+
+def test_decode_shared_without_a_prefix_page():
+    """A prefix table without columns: the sequences' own rows are all there is."""
+    from gemq_b200.kernels import latent_decode_shared
+    q_latent, q_rope, cache, table, n, rows = decode_case([100, 30, 0], 2, 16, 512, 64, torch.float16)
+    none, starts = torch.zeros(2, dtype=torch.int32, device="cuda"), torch.tensor([0, 2, 3], dtype=torch.int32, device="cuda")
+    got = latent_decode_shared(q_latent, q_rope, cache, table, n, torch.zeros(2, 0, dtype=torch.int32, device="cuda"), none, starts, 0.07)
+    check_decode(*got, q_latent, q_rope, [rows_of(cache, r) for r in rows], 0.07)
+    same = latent_decode_shared(q_latent, q_rope, cache, table, n, torch.zeros(2, 5, dtype=torch.int32, device="cuda"), none, starts, 0.07)
+    assert all(torch.equal(a, b) for a, b in zip(got, same))
