@@ -99,6 +99,7 @@ _SIGNATURES = {
     "gemq_latent_decode_scratch_bytes": (_Z, [C.POINTER(LatentDecode)]),
     "gemq_latent_decode": (_I, [C.POINTER(LatentDecode), _P, _Z, _P]),
     "gemq_latent_prefill": (_I, [C.POINTER(LatentPrefill), _P]),
+    "gemq_latent_take_error": (_I, [_P, _P, _P]),
     "gemq_copy_pages": (_I, [_P, _L, _L, _I, _I, _L, _P, _P, _I, _P, _P]),
     "gemq_moe_decode": (_I, [C.POINTER(MoeLayer), _P, _P, _P, _P, _I, _I, _I, _P, _Z, _P]),
 }

@@ -176,10 +176,18 @@ __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const CopyArgs
   }
 }
 
+__global__ void take_error_kernel(int* err, int* code) { *code = atomicExch(err, 0); }
+
 }  // namespace
 }  // namespace gemq
 
 using namespace gemq;
+
+extern "C" int gemq_latent_take_error(int32_t* err, int32_t* code, gemq_stream_t stream) {
+  if (!err || !code) return GEMQ_ERR_BAD_ARG;
+  take_error_kernel<<<1, 1, 0, static_cast<cudaStream_t>(stream)>>>(err, code);
+  return launch_status();
+}
 
 extern "C" int gemq_latent_append(const void* kv, int64_t kv_stride, const void* q_rope, int64_t q_token_stride, int64_t q_head_stride,
                                   const void* norm_weight, float eps, const float* inv_freq, float rope_scale, const int64_t* positions,

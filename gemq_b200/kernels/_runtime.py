@@ -64,17 +64,26 @@ def check_kernel_form(wq, scales, zeros, K: int, N: int, nbits: int, group_size:
 _err_words: dict = {}
 
 
-def error_word(dev: torch.device) -> torch.Tensor:
-    """One int32 per device that kernels with bounded waits set when a wait expires."""
+def _error_words(dev: torch.device):
     key = (dev.type, dev.index if dev.index is not None else torch.cuda.current_device())
     t = _err_words.get(key)
     if t is None:
-        t = torch.zeros(1, dtype=torch.int32, device=dev)
-        _err_words[key] = t
+        t = _err_words[key] = torch.zeros(2, dtype=torch.int32, device=dev).split(1)  # both are there once one is
     return t
 
 
+def error_word(dev: torch.device) -> torch.Tensor:
+    """One int32 per device that kernels with bounded waits set when a wait expires."""
+    return _error_words(dev)[0]
+
+
+def latent_error_word(dev: torch.device) -> torch.Tensor:
+    """The latent operators' own, as what they report is taken and cleared by itself."""
+    return _error_words(dev)[1]
+
+
 _err_ptrs: dict = {}
+_latent_err_ptrs: dict = {}
 
 
 def host_error_word(x):
@@ -83,6 +92,14 @@ def host_error_word(x):
     p = _err_ptrs.get(i)
     if p is None and i >= 0:
         p = _err_ptrs[i] = error_word(x.device).data_ptr()
+    return p
+
+
+def host_latent_error_word(x):
+    i = x.get_device()
+    p = _latent_err_ptrs.get(i)
+    if p is None and i >= 0:
+        p = _latent_err_ptrs[i] = latent_error_word(x.device).data_ptr()
     return p
 
 

@@ -8,8 +8,8 @@ A token is cached as one row of ``rank + 64`` numbers that all heads share: the 
 of the key.  A cache is ``[pages, page_size, rank + 64]``, fp16 or bf16, any stride between pages; ``page_size`` is 16, 32 or a
 multiple of 64, ``rank`` 128, 256, 384 or 512.  Lengths, page tables and slots are device tensors that no call reads on the host,
 so every call can be captured in a CUDA graph.  Entries out of range are reported in the device's error word
-(``gemq_b200.kernels.latent_error``) and never used as an index.  That word is made by the first call on a device, which belongs
-outside a capture.  Serving only: the operators have no gradients.
+(``gemq_b200.kernels.latent_error``) and never used as an index.  That word is made by the first call of this package on a device, which
+belongs outside a capture.  Serving only: the operators have no gradients.
 """
 from __future__ import annotations
 
@@ -21,7 +21,7 @@ from torch import Tensor
 
 from .. import _capi
 from ._ops import library_op
-from ._runtime import error_word, host_error_word, require, require_cuda, stream_ptr
+from ._runtime import host_latent_error_word, latent_error_word, require, require_cuda, stream_ptr
 
 ROPE, NOPE, VALUE = 64, 128, 128
 _HALF = (torch.float16, torch.bfloat16)
@@ -45,20 +45,24 @@ class _on:
 def _native(name: str):
     """The call in native code (csrc/host.cpp); None where it does not take the arguments, which the checks here then name."""
     def fast(x, *rest):
-        p = host_error_word(x) if isinstance(x, Tensor) else None
+        p = host_latent_error_word(x) if isinstance(x, Tensor) else None
         return None if p is None else getattr(_capi.host, name)(p, x, *rest)
     return fast
 
 
 def latent_error(device=None) -> int:
     """The code of what the latent operators found out of range on the device since the last call of this, 0 for nothing:
-    41 page, 42 length or offsets, 43 slot, 44 a wait inside a kernel.  Waits for the device."""
-    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-    word = error_word(dev)
-    code = int(word.item())
-    if code:
-        word.zero_()
-    return code
+    41 page, 42 length or offsets, 43 slot, 44 a wait inside a kernel; of several the latest.  Waits for all streams of the device; the
+    code is taken and cleared at once, so what calls that run meanwhile report is left for the next call."""
+    dev = torch.device("cuda") if device is None else torch.device(device)
+    require(dev.type == "cuda", f"the latent operators run on CUDA devices, not on {dev}")
+    if dev.index is None:
+        dev = torch.device(dev.type, torch.cuda.current_device())
+    torch.cuda.synchronize(dev)
+    code = torch.empty(1, dtype=torch.int32, device=dev)
+    with _on(dev):
+        _capi.check("gemq_latent_take_error", _capi.lib.gemq_latent_take_error(latent_error_word(dev).data_ptr(), code.data_ptr(), stream_ptr(dev)))
+    return int(code.item())
 
 
 def _strides(name: str, t: Tensor) -> list:
@@ -122,7 +126,7 @@ def latent_append(kv: Tensor, q_rope: Tensor, norm_weight: Tensor, eps: float, i
         _capi.check("gemq_latent_append", _capi.lib.gemq_latent_append(
             kv.data_ptr(), kv_stride, q_rope.data_ptr() if H else None, *q_strides, norm_weight.data_ptr(), eps, inv_freq.data_ptr(),
             rope_scale, positions.data_ptr(), slots.data_ptr(), cache.data_ptr(), page_stride, cache.shape[0], cache.shape[1], rows.data_ptr(),
-            q_out.data_ptr() if H else None, T, H, rank, int(kv.dtype == torch.bfloat16), error_word(dev).data_ptr(), stream_ptr(dev)))
+            q_out.data_ptr() if H else None, T, H, rank, int(kv.dtype == torch.bfloat16), latent_error_word(dev).data_ptr(), stream_ptr(dev)))
     return q_out, rows
 
 
@@ -157,7 +161,7 @@ def _decode(q_latent, q_rope, cache, table, lens, scale, prefix_table=None, pref
     A.cache, A.page_stride, A.n_pages, A.page_size = cache.data_ptr(), page_stride, cache.shape[0], cache.shape[1]
     A.table, A.table_pitch, A.lens = table.data_ptr() or cache.data_ptr(), table.shape[1], lens.data_ptr()
     A.batch, A.steps, A.heads, A.rank, A.scale, A.is_bf16 = B, S, H, rank, scale, int(q_latent.dtype == torch.bfloat16)
-    A.out, A.lse, A.err = out.data_ptr(), lse.data_ptr(), error_word(dev).data_ptr()
+    A.out, A.lse, A.err = out.data_ptr(), lse.data_ptr(), latent_error_word(dev).data_ptr()
     with _on(dev):
         n = _capi.lib.gemq_latent_decode_scratch_bytes(C.byref(A))
         scratch = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
@@ -242,7 +246,7 @@ def latent_prefill(q_nope: Tensor, q_rope: Tensor, kv: Tensor, k_rope: Tensor, c
         A.k_rope, A.k_rope_stride = k_rope.data_ptr(), _strides("k_rope", k_rope)[0]
     A.cu_q, A.cu_k, A.batch, A.q_rows, A.k_rows = cu_q.data_ptr(), cu_k.data_ptr(), cu_q.shape[0] - 1, Tq, Tk
     A.heads, A.causal, A.scale, A.is_bf16 = H, int(causal), scale, int(q_nope.dtype == torch.bfloat16)
-    A.out, A.lse, A.err = out.data_ptr(), lse.data_ptr(), error_word(dev).data_ptr()
+    A.out, A.lse, A.err = out.data_ptr(), lse.data_ptr(), latent_error_word(dev).data_ptr()
     with _on(dev):
         _capi.check("gemq_latent_prefill", _capi.lib.gemq_latent_prefill(C.byref(A), stream_ptr(dev)))
     return out, lse
@@ -276,4 +280,4 @@ def copy_pages(cache: Tensor, src: Tensor, dst: Tensor) -> None:
     with _on(dev):
         _capi.check("gemq_copy_pages", _capi.lib.gemq_copy_pages(
             cache.data_ptr(), layer_stride * size, page_stride * size, layers, cache.shape[-page.dim() - 1], nbytes, src.data_ptr(), dst.data_ptr(),
-            src.numel(), error_word(dev).data_ptr(), stream_ptr(dev)))
+            src.numel(), latent_error_word(dev).data_ptr(), stream_ptr(dev)))

@@ -329,6 +329,9 @@ enum {
   GEMQ_LATENT_WAIT = 44        /* a wait inside a kernel ran out */
 };
 
+/* *code = *err, *err = 0, as one exchange on the device: a code that a kernel of another stream reports meanwhile is not lost. */
+int gemq_latent_take_error(int32_t* err, int32_t* code, gemq_stream_t stream);
+
 /* rows [tokens, rank + 64] = { RMSNorm(kv[:, :rank]) * norm_weight, kv[:, rank:] rotated }, each rounded once to T, also stored at row
  * slots[t] (page slots[t] / page_size; slots[t] < 0: not stored, -1 silently) of the cache; q_out [tokens, heads, 64] = q_rope rotated.
  * Rotation of the pair (x[2i], x[2i+1]) by the angle positions[t] * inv_freq[i], formed in 64 bits, times rope_scale.  The strides

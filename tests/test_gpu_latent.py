@@ -612,3 +612,31 @@ def test_decode_shared_without_a_prefix_page():
     check_decode(*got, q_latent, q_rope, [rows_of(cache, r) for r in rows], 0.07)
     same = latent_decode_shared(q_latent, q_rope, cache, table, n, torch.zeros(2, 5, dtype=torch.int32, device="cuda"), none, starts, 0.07)
     assert all(torch.equal(a, b) for a, b in zip(got, same))
+
+
+# ---- what is reported ---------------------------------------------------------------------------------
+def test_errors_are_the_latent_operators_own():
+    """A code that the linears' waits left in their word is neither returned nor cleared."""
+    from gemq_b200.kernels import copy_pages, latent_error
+    from gemq_b200.kernels._runtime import error_word
+    word = error_word(torch.device("cuda", torch.cuda.current_device()))
+    assert int(word.item()) == 0
+    try:
+        word.fill_(7)
+        assert latent_error() == 0 and int(word.item()) == 7
+        copy_pages(torch.zeros(2, 4, 2, 8, device="cuda"), torch.tensor([9], device="cuda"), torch.tensor([1], device="cuda"))
+        assert int(word.item()) == 7 and latent_error("cuda") == 41 and latent_error() == 0
+    finally:
+        word.zero_()
+
+
+def test_errors_of_other_streams_are_waited_for():
+    from gemq_b200.kernels import copy_pages, latent_error
+    cache, src, dst = torch.zeros(2, 4, 2, 8, device="cuda"), torch.tensor([9], device="cuda"), torch.tensor([1], device="cuda")
+    side = torch.cuda.Stream()
+    for _ in range(3):  # the first loads the kernels, which waits by itself
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(200_000_000)  # a tenth of a second
+            copy_pages(cache, src, dst)
+        assert latent_error() == 41 and latent_error() == 0

@@ -292,3 +292,9 @@ def test_attention_layer_follows_its_weights():
     assert torch.equal(a.w_keys, w[:, :128]) and torch.equal(a.w_values, w[:, 128:].transpose(1, 2)) and torch.equal(a.norm_weight, b.norm_weight)
     a.half()
     assert a.w_keys.dtype == a.norm_weight.dtype == f16 and a.inv_freq.dtype == torch.float32
+
+
+def test_taking_an_error_refuses():
+    assert _capi.lib.gemq_latent_take_error(None, 1 << 20, None) == -1 and _capi.lib.gemq_latent_take_error(1 << 20, None, None) == -1
+    with pytest.raises(ValueError, match="CUDA"):
+        K.latent_error("cpu")
