@@ -128,7 +128,7 @@ class _NoHost:
     linked to the one next to it): every call goes through ctypes."""
 
     plain = linear = moe_decode = moe_prefill = staticmethod(lambda *a: None)
-    latent_decode = latent_prefill = latent_append = copy_pages = plain
+    latent_decode = latent_prefill = latent_append = copy_pages = written = plain
 
 
 if os.environ.get("GEMQ_B200_LIB"):

@@ -9,6 +9,7 @@ plus the C-ABI call on the current stream -- runs at execution (and CUDA-graph c
 from __future__ import annotations
 
 import functools
+import inspect
 
 import torch
 from torch.autograd import forward_ad
@@ -54,21 +55,25 @@ def library_op(name: str, fake, fast=None, mutates=()):
     A call in eager mode goes straight to ``fn``: the Python dispatch of a custom operator costs
     20-30 us of host time, more than the kernels of a small call take.  ``fast`` is tried before it with the
     positional arguments: native code that returns None for what it does not take.  Every other call
-    (``plain_call``) is the operator."""
+    (``plain_call``) is the operator.  What is written counts as written for autograd on either way: a gradient
+    that was to come from its old contents is refused."""
     def deco(fn):
         op = torch.library.custom_op(f"{NAMESPACE}::{name}", mutates_args=mutates)(fn)
         op.register_fake(fake)
         overload = op._opoverload
+        written = [(list(inspect.signature(fn).parameters).index(m), m) for m in mutates]
 
         @functools.wraps(fn)
         def call(*args, **kwargs):
             if not plain_call(*args, *kwargs.values()):
                 return overload(*args, **kwargs)
-            if fast is not None and not kwargs:
-                y = fast(*args)
-                if y is not None:
-                    return y
-            return fn(*args, **kwargs)
+            y = fast(*args) if fast is not None and not kwargs else None
+            if y is None:
+                y = fn(*args, **kwargs)
+            for i, m in written:
+                t = args[i] if i < len(args) else kwargs[m]
+                _capi.host.written(t) or torch.autograd.graph.increment_version(t)
+            return y
 
         call._init_fn = fn
         for method in ("register_autograd", "register_fake", "register_kernel", "register_vmap"):

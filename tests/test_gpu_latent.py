@@ -640,3 +640,30 @@ def test_errors_of_other_streams_are_waited_for():
             torch.cuda._sleep(200_000_000)  # a tenth of a second
             copy_pages(cache, src, dst)
         assert latent_error() == 41 and latent_error() == 0
+
+
+# ---- writes into the cache ------------------------------------------------------------------------------
+def test_writes_into_the_cache_are_seen_by_autograd():
+    """What a differentiable product has kept of the cache, and an operator then overwrote, is not used for a gradient."""
+    from gemq_b200.kernels import copy_pages, latent_append
+    cache = torch.ones(2, 64, 576, dtype=torch.float16, device="cuda")
+    kv, w, i64 = torch.ones(1, 576, dtype=torch.float16, device="cuda"), torch.ones(512, dtype=torch.float16, device="cuda"), torch.int64
+    slot, page = torch.zeros(1, dtype=i64, device="cuda"), torch.ones(1, dtype=i64, device="cuda")
+    append = lambda c: latent_append(kv, kv[:, None, :64], w, 1e-6, torch.ones(32, device="cuda"), slot, slot, c)  # noqa: E731
+    for name, write in (("native", append), ("no heads", lambda c: latent_append(kv, kv[:, None, :64][:, :0], w, 1e-6, torch.ones(32, device="cuda"), slot, slot, c)),
+                        ("by name", lambda c: latent_append(kv, kv[:, None, :64], w, 1e-6, torch.ones(32, device="cuda"), slot, slot, cache=c)),
+                        ("one layer", lambda c: copy_pages(c, slot, page)), ("layers", lambda c: copy_pages(c.view(1, 2, 64, 576), slot, page)),
+                        ("pages by name", lambda c: copy_pages(src=slot, dst=page, cache=c))):
+        before = cache._version
+        write(cache)
+        assert cache._version > before, name
+        x = torch.ones(576, dtype=torch.float16, device="cuda", requires_grad=True)
+        y = (cache[0] * x).sum()
+        write(cache)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    with torch.inference_mode():
+        c = torch.ones(2, 64, 576, dtype=torch.float16, device="cuda")
+        append(c)
+        copy_pages(c, slot, page)
+        assert torch.equal(c[0], c[1])
