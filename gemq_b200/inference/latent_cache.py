@@ -146,6 +146,8 @@ class PagedLatentCache:
     def plan_decode(self, seqs: Sequence[int], steps: int = 1, groups: Optional[Sequence[int]] = None) -> LatentPlan:
         """``steps`` new rows for every sequence.  ``groups`` gives the number of sequences of each group that may share a prefix: the pages that all of
         a group begin with are then read once (``latent_decode_shared``)."""
+        if steps < 1:
+            raise ValueError(f"a decode step has one new row a sequence at least, not {steps}")
         if groups is not None and (sum(groups) != len(seqs) or any(g <= 0 for g in groups) or not groups):
             raise ValueError("groups must cover the sequences, one or more in each")
         slots = self.extend(seqs, [steps] * len(seqs))

@@ -298,3 +298,13 @@ def test_taking_an_error_refuses():
     assert _capi.lib.gemq_latent_take_error(None, 1 << 20, None) == -1 and _capi.lib.gemq_latent_take_error(1 << 20, None, None) == -1
     with pytest.raises(ValueError, match="CUDA"):
         K.latent_error("cpu")
+
+
+def test_a_decode_plan_has_a_step(cache):
+    """None would be the plan of a prefill; nothing is taken by a refused one."""
+    a = cache.new()
+    cache.extend([a], [20])
+    for steps in (0, -1):
+        with pytest.raises(ValueError, match="step"):
+            cache.plan_decode([a], steps)
+    assert cache.length(a) == 20 and cache.free_pages == 10
