@@ -24,6 +24,10 @@ def _weight(linear, dtype: torch.dtype) -> Tensor:
     return linear.weight.to(dtype)
 
 
+def _refresh(layer: "LatentAttention", _) -> None:  # a function of the module: the layer can be pickled
+    layer.refresh()
+
+
 class LatentAttention(nn.Module):
     """``q_proj`` (any module from hidden states to ``heads * 192``), ``kv_a_proj`` (to ``rank + 64``), the latent's norm weight and ``kv_b_proj``
     (from ``rank`` to ``heads * 256``), ``o_proj`` (from ``heads * 128``).  Prompts are attended to in the expanded form, decoded tokens
@@ -45,7 +49,7 @@ class LatentAttention(nn.Module):
         self.inv_freq = inv_freq.detach().float().contiguous()  # no buffer: a change of the module's type leaves it in 32 bits
         self.rank = rank
         self.refresh()
-        self.register_load_state_dict_post_hook(lambda module, _: module.refresh())
+        self.register_load_state_dict_post_hook(_refresh)
 
     def refresh(self) -> None:
         """The halves of ``kv_b_proj``'s weight as it is now."""

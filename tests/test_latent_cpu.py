@@ -308,3 +308,20 @@ def test_a_decode_plan_has_a_step(cache):
         with pytest.raises(ValueError, match="step"):
             cache.plan_decode([a], steps)
     assert cache.length(a) == 20 and cache.free_pages == 10
+
+
+def test_attention_layer_is_saved_whole():
+    """Pickled, copied, and still following the weights that are loaded into it."""
+    import copy
+    import io
+    from gemq_b200.inference import LatentAttention
+    make = lambda: LatentAttention(*(torch.nn.Linear(i, o, bias=False) for i, o in ((32, 768), (32, 192))), torch.rand(128), 1e-6,  # noqa: E731
+                                   torch.nn.Linear(128, 1024, bias=False), torch.nn.Linear(512, 32, bias=False), 4, torch.rand(32))
+    a, b = make(), make()
+    file = io.BytesIO()
+    torch.save(torch.nn.Sequential(a), file)
+    file.seek(0)
+    for c in (torch.load(file, weights_only=False)[0], copy.deepcopy(a)):
+        assert torch.equal(c.w_keys, a.w_keys) and torch.equal(c.inv_freq, a.inv_freq) and c.scale == a.scale
+        c.load_state_dict(b.state_dict())
+        assert torch.equal(c.w_keys, b.w_keys) and torch.equal(c.w_values, b.w_values) and not torch.equal(a.w_keys, b.w_keys)
