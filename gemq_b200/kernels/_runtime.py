@@ -106,9 +106,11 @@ def host_latent_error_word(x):
 def host_linear(x, w_q, scales, zeros, nbits, group_size, bias, mode: int):
     """The native call (csrc/host.cpp) or None.  ``mode``: 0 dense layer, 1 rows operator, 2 one-row operator,
     3 GEMM operator."""
-    p = host_error_word(x)
+    p = _err_ptrs.get(x.get_device())
     if p is None:
-        return None
+        p = host_error_word(x)
+        if p is None:
+            return None
     return _capi.host.linear(x, w_q, scales, zeros, nbits, group_size, bias, p, mode)
 
 
