@@ -667,3 +667,41 @@ def test_writes_into_the_cache_are_seen_by_autograd():
         append(c)
         copy_pages(c, slot, page)
         assert torch.equal(c[0], c[1])
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_copy_pages_of_one_layer(native):
+    """The forms without a dimension for the layers, pages further apart than they are long; four dimensions beside them, in both routes."""
+    from gemq_b200.kernels import copy_pages
+    gen = generator(5)
+    src, dst = torch.tensor([4, 0, 4, 8], device="cuda"), torch.tensor([1, 2, 7, 8], device="cuda")
+    for big, view in ((torch.randn(9, 3, 4, 24, device="cuda", generator=gen), lambda t: t[:, 1]),      # [9, 4, 24], 288 apart
+                      (torch.randn(9, 40, device="cuda", generator=gen), lambda t: t[:, 8:28]),          # [9, 20], 40 apart
+                      (torch.randn(18, 8, 16, device="cuda", generator=gen).half(), lambda t: t[::2]),
+                      (torch.randn(3, 9, 2, 5, 8, device="cuda", generator=gen), lambda t: t[:, :, 1]),  # layers
+                      (torch.randn(9, 3, 5, 8, device="cuda", generator=gen), lambda t: t.transpose(0, 1))):
+        want = big.clone()
+        dim = 1 if view(big).dim() >= 4 else 0
+        view(want).index_copy_(dim, dst, view(big).index_select(dim, src))
+        if native:
+            copy_pages(view(big), src, dst)
+        else:
+            torch.ops.gemq_b200.copy_pages(view(big), src, dst)
+        assert torch.equal(big, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("prefix,sizes,own,S,H,R,page", [
+    ([200], [3], [1, 64, 100], 1, 5, 512, 64),          # 15 rows in the batch
+    ([90, 0], [1, 1], [30, 7], 2, 4, 256, 16),          # 16
+    ([1000], [4], [1, 0, 40], 1, 8, 512, 32),           # 32
+    ([300, 70], [2, 1], [5, 200], 3, 3, 128, 64),       # 27
+    ([40000], [2], [1, 100], 1, 16, 512, 64),           # 32, a prefix over all CTAs
+])
+def test_decode_shared_of_few_rows(prefix, sizes, own, S, H, R, page, dtype):
+    test_decode_shared(prefix, sizes, own, S, H, R, page, dtype)
+
+
+@pytest.mark.parametrize("lens,S,H,page", [([131072], 1, 16, 64), ([131071, 3, 131072], 2, 16, 16), ([200001, 70], 1, 64, 128)])
+def test_decode_of_far_positions(lens, S, H, page):
+    test_decode(lens, S, H, 512, page, torch.bfloat16)
