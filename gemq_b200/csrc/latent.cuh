@@ -75,7 +75,7 @@ __device__ __forceinline__ void wait_for(unsigned long long* bar, uint32_t parit
   else wait_here(smem_u32(bar), parity, abort, err);
 }
 
-// Division of a 32-bit n >= 0 by a number of the launch: with l = ceil(log2 d) the multiplier floor(2^32 (2^l - d) / d) + 1 and 2^32 above it
+// Division of a 32-bit n >= 0 by a number of the launch (Granlund and Montgomery, "Division by invariant integers using multiplication", 1994): with l = ceil(log2 d) the multiplier floor(2^32 (2^l - d) / d) + 1 and 2^32 above it
 // give n / d after a shift by l, the sum halved on the way so that it fits.
 struct Div {
   uint32_t mul;

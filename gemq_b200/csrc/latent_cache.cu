@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(32 * kAppendWarps) latent_append_kernel(const 
   for (int i = 0; i < 2; ++i) v[i] = lane + 32 * i < pieces ? src[lane + 32 * i] : make_uint4(0, 0, 0, 0);
   const uint32_t kp = reinterpret_cast<const uint32_t*>(src + pieces)[lane];
 
-  // the first 16 heads' queries are asked for here: eight lanes a head, four pairs a lane
+  // the first 16 heads' queries are asked for here: eight lanes a head, four pairs a lane (those of more heads behind the norm)
   const T* q = static_cast<const T*>(P.q) + t * P.q_token + (lane & 7) * 8;
   uint4 early[4];
 #pragma unroll

@@ -19,12 +19,13 @@
 //                ring for it.)
 //   warps 4-7    softmax (a thread has two positions x N / 4 rows), O's correction
 //   warps 8-11   the queries of the next piece into shared memory, results of the last
-// The maximum that the weights refer to moves only when a row's scores exceed it by 2^8: O is corrected in tensor memory a few times per
-// sequence.  Rows behind what is seen are zeroed in shared memory before they are multiplied by weights of 0: what lies there may be NaN.
+// The maximum that a row's weights refer to moves only when its own scores exceed it by 2^8: O is corrected in tensor memory a few times per
+// sequence, and no row's bits depend on what others of its tile hold or see.  Weights are rounded to the type for the second product, their sums are
+// not: as 16 bits are what the product takes, and the logarithm of the sum keeps all of its own.  Rows behind what is seen are zeroed in shared memory before they are multiplied by weights of 0: what lies there may be NaN.
 // Every wait is bounded.
 //
-// Measured (rank 512; the call with both launches): 37 sequences of 60 to 9000 positions, 16 heads, 80 MB: 33 us, 2.4 TB/s; 2 sequences of 70,001
-// and 131,072, 48 rows each, 232 MB: 65 us, 3.6 TB/s; 64 sequences behind a prefix of 8000, 18 GFLOP: 48 us; one of 700: 11 us.  A CTA's 64
+// Measured (rank 512; the call with both launches): 37 sequences of 60 to 9000 positions, 16 heads, 80 MB: 35 us, 2.3 TB/s; 2 sequences of 70,001
+// and 131,072, 48 rows each, 232 MB: 67 us, 3.5 TB/s; 64 sequences behind a prefix of 8000, 18 GFLOP: 50 us; one of 700: 11.5 us.  A CTA's 64
 // positions take 3100 to 3300 cycles with all SMs at work: 16 rows what HBM gives (3100), 64 rows the two products' reads of shared memory
 // (2000 cycles of MMAs, 340 KB at 128 bytes a cycle) and a ring of two tiles.  The rest is fixed: 3 to 5 us to the first copy, 3 to the first
 // weights, 1 to 4 for results (64 rows: 131 KB at 32 bytes a cycle), 2 to 6 for the join.
@@ -109,7 +110,8 @@ __device__ __forceinline__ Entry entry_here(const Args& P, int e) {
     x.len = clamp_length(A.lens[b], A.table_pitch, A.page_size, A.err);
   }
   x.tiles = cdiv(x.len, kTile);
-  // Measured, two and more pieces of a CTA against one: 16 rows 3.4 us a piece and 2.2 a tile, 64 rows 4 us and 1.7.
+  // Measured at rank 512, two and more pieces of a CTA against one: 16 rows 3.4 us a piece and 2.2 a tile, 64 rows 4 us and 1.7.  (A tile of a lower
+  // rank is shorter beside its piece: shares are less even there.)
   x.piece = x.rows <= 32 ? 6 : 9;
   x.cost = x.tiles ? 4 * x.tiles + x.piece : 0;
   return x;
@@ -898,7 +900,11 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
 // ---- pieces of a row joined ---------------------------------------------------------------------------
 // A warp has 128 numbers of a row, eight pieces in flight.  Many rows have few pieces each (W = 1): a CTA has a row, and its warps all pieces of
 // their numbers.  Few rows may have a piece from every CTA (W = 8): a CTA has 128 numbers, its warps take every eighth piece and keep a maximum
-// of their own; the eight are added in a fixed order.
+// of their own; the eight are added in a fixed order.  What decides is the pieces a row, which only the device knows; the rows of the batch stand in
+// for it: up to two a CTA take W = 8.  Measured, the call in a graph, 16 heads, W = 8 against W = 1: one sequence of 200,000 positions 52 and 81 us;
+// 20,000 positions in 4 equal ones 14.6 and 22.2, in 9 17.8 and 19.5, in 18 22.1 and 17.7, in 37 30.6 and 17.5; one of 131,072 beside 19 of 200
+// 43 and 70.  Equal lengths alone would put the line at 10 sequences; it stands where a batch of 18 loses 4 us if they are equal and gains 27 if one
+// of them is long.
 constexpr int kJoinAhead = 8;
 
 template <typename T, int W>

@@ -13,7 +13,8 @@
 //               250 to 600 cycles between any two products.)
 //   warp 3      a second pass only, see below
 //   warps 4-7, 8-11   softmax of either tile, results
-// The reference of a row's weights moves only when its scores exceed it by 2^8; then its sums are corrected in tensor memory.
+// The reference of a row's weights moves only when its own scores exceed it by 2^8; then its sums are corrected in tensor memory.  Weights are
+// rounded to the type for the second product, their sums are not (the logarithm of the sum keeps all of its bits).
 //
 // What a query must not see is given a weight of 0.  If such a row of v holds an infinity or a NaN the product still is NaN: a block with a
 // result that is not finite is computed once more, and warp 3 sets to zero, in the tiles that not all of its queries see whole, what

@@ -10,6 +10,10 @@ multiple of 64, ``rank`` 128, 256, 384 or 512.  Lengths, page tables and slots a
 so every call can be captured in a CUDA graph.  Entries out of range are reported in the device's error word
 (``gemq_b200.kernels.latent_error``) and never used as an index.  That word is made by the first call of this package on a device, which
 belongs outside a capture.  Serving only: the operators have no gradients.
+
+The attention operators form scores, maxima, sums and results in 32 bits.  Each weight is rounded once to the type of the cache for the product
+with the values (off by half a step of it at most, fp16 2^-11, bf16 2^-8, relative to the weight), their sum is not; results are
+rounded once more.
 """
 from __future__ import annotations
 
@@ -52,8 +56,8 @@ def _native(name: str):
 
 def latent_error(device=None) -> int:
     """The code of what the latent operators found out of range on the device since the last call of this, 0 for nothing:
-    41 page, 42 length or offsets, 43 slot, 44 a wait inside a kernel; of several the latest.  Waits for all streams of the device; the
-    code is taken and cleared at once, so what calls that run meanwhile report is left for the next call."""
+    41 page, 42 length or offsets, 43 slot, 44 a wait inside a kernel; of several the latest.  Waits for all streams of the device (not
+    while one of them is captured); the code is taken and cleared at once, so what calls that run meanwhile report is left for the next call."""
     dev = torch.device("cuda") if device is None else torch.device(device)
     require(dev.type == "cuda", f"the latent operators run on CUDA devices, not on {dev}")
     if dev.index is None:
